@@ -36,6 +36,7 @@ extern "C" {
 
 #define UOCR_HIP_DTYPE_F32 0
 #define UOCR_HIP_DTYPE_BF16 1
+#define UOCR_HIP_DTYPE_F16 2 /* paged attention and rotary positions only */
 
 /* Error text of the calling thread's most recent failing call ("" if none). */
 const char* uocr_hip_last_error(void);
@@ -481,6 +482,134 @@ int uocr_hip_rswa_write_prefill_ragged(const float* k, const float* v, float* kc
 int uocr_hip_rswa_attention_ragged(const float* q, const float* kcache_base, const float* vcache_base,
                                    const int* d_slots, const int* d_pos, int total, int batch_cap, int heads,
                                    int kv_heads, int head_dim, float* out, void* stream);
+
+/* ---- Rotary positions, paged KV cache and its attention (no counterpart in
+ * the reference, whose cache is one contiguous f32 block per request) ----
+ * Descriptors are host structs, read during the call; the pointers in them are
+ * device pointers unless said otherwise. Strides are in elements.
+ *
+ * Rows of heads: element d of head h of row t is data[t * row_stride +
+ * h * head_stride + d], so q, k and v may be columns of one projection's output. */
+typedef struct {
+    void* data;
+    int dtype; /* UOCR_HIP_DTYPE_F32, _BF16 or _F16 */
+    long long row_stride, head_stride;
+} uocr_hip_rows;
+
+/* Cache: row r of page p of KV head h starts at p * page_stride + r * row_stride +
+ * h * head_stride of k and of v; any order of the three, e.g.
+ * [n_pages, page_size, kv_heads, head_dim]. Row j of sequence s is row
+ * j % page_size of page page_table[s * table_stride + j / page_size].
+ * Requirements: head_dim a multiple of 8 up to 256, k and v 16-byte aligned, strides
+ * multiples of 16 bytes and not negative. Entries of the table for rows that a call neither writes
+ * nor sees are not read, so pages that left a window may be given to others
+ * (set the entry to anything). */
+typedef struct {
+    void* k;
+    void* v;
+    int dtype;
+    int n_pages, page_size, kv_heads, head_dim;
+    long long page_stride, row_stride, head_stride;
+    const int* page_table;
+    int n_seqs, max_pages;
+    long long table_stride;
+} uocr_hip_paged_cache;
+
+/* Rotary frequencies, on the host, in 64 bits rounded once: inv_freq[i] for
+ * i < rotary_dim / 2 and *factor, the factor on cos and sin.
+ *   NONE    base^(-2i / rotary_dim)
+ *   LINEAR  the same / factor_len (positions interpolated; Chen et al. 2023, arXiv:2306.15595)
+ *   BASE    base * factor_len^(rotary_dim / (rotary_dim - 2)) instead of base
+ *   PARTS   per frequency: kept above `fast` turns over original_len positions,
+ *           divided by factor_len below `slow` turns, a linear ramp over i between;
+ *           *factor = 0.1 ln(factor_len) + 1 (Peng et al. 2023, arXiv:2309.00071)
+ * factor_len >= 1; original_len, fast > slow > 0 for PARTS (ignored elsewhere). */
+enum {
+    UOCR_HIP_ROPE_NONE = 0,
+    UOCR_HIP_ROPE_LINEAR = 1,
+    UOCR_HIP_ROPE_BASE = 2,
+    UOCR_HIP_ROPE_PARTS = 3
+};
+int uocr_hip_rope_frequencies(int rotary_dim, double base, int scaling, double factor_len, int original_len,
+                              double fast, double slow, float* inv_freq /* host */, float* factor /* host */);
+
+/* Rotary positions: q_out, k_out = q, k with the first rotary_dim dims of every
+ * head of row t turned by the angles positions[t] * inv_freq[i]: pair i is
+ * (i, i + rotary_dim / 2), or (2i, 2i + 1) if interleaved; (a, b) becomes
+ * factor * (a cos - b sin, b cos + a sin). The other dims are copied. Angles
+ * are reduced in 64 bits (any int position), the rest is f32, rounded once.
+ * q_out may be q (the same strides and type), k_out k; other overlaps are not
+ * allowed. Input and output types may differ (q and k share theirs, as do q_out and
+ * k_out). k and k_out may be NULL (kv_heads 0). rotary_dim even, 0..head_dim. */
+int uocr_hip_rope(const uocr_hip_rows* q, const uocr_hip_rows* k, int rows, int heads, int kv_heads, int head_dim,
+                  const int* positions, const float* inv_freq, int rotary_dim, int interleaved, float factor,
+                  const uocr_hip_rows* q_out, const uocr_hip_rows* k_out, void* stream);
+
+/* The same with the append to the cache in the same pass: row t's rotated k
+ * and its v, rounded to the cache's type, become row d_rows[t] of sequence
+ * d_seqs[t]; q_out gets the rotated q. rotary_dim 0 appends without rotation
+ * (positions and inv_freq may be NULL). A row whose d_seqs[t] is not in [0, n_seqs) is padding:
+ * nothing of it is read or written, q_out included. A row whose d_rows[t] is outside the table,
+ * or whose page is not in [0, n_pages), is not stored (attention that sees it gives NaN). Of several
+ * rows that name the same place one ends up there, each element from one of them. */
+int uocr_hip_rope_append_paged(const uocr_hip_rows* q, const uocr_hip_rows* k, const uocr_hip_rows* v, int rows,
+                               int heads, const int* positions, const float* inv_freq, int rotary_dim,
+                               int interleaved, float factor, const uocr_hip_paged_cache* cache, const int* d_seqs,
+                               const int* d_rows, const uocr_hip_rows* q_out, void* stream);
+
+/* Scores and masks of the paged attention. With p the position of a query row and j that of a key:
+ *   score = scale * q.k, then softcap * tanh(score / softcap) if softcap > 0,
+ *           then - slopes[head] * |p - j| if slopes
+ *   seen    j < kv_len, key_begin[row] <= j < key_end[row], and
+ *           (causal: j <= p; window: j > p - window), or j < prefix_len[seq]
+ *           (and j <= p too, unless prefix_both_ways or not causal)
+ * window with prefix_len is the R-SWA set: the first rows and the last ones.
+ * A document mask is key_begin (and key_end where not causal). A row that sees nothing gives zeros.
+ * What is not seen has no influence, whatever its values (NaN and infinities included). */
+typedef struct {
+    int heads;             /* query heads, a multiple of the cache's kv_heads */
+    float scale;           /* 0: 1 / sqrt(head_dim) */
+    float softcap;         /* 0: none */
+    const float* slopes;   /* [heads] f32 or NULL */
+    int causal;            /* prefill only (a single new token sees no later key) */
+    int window;            /* 0: none; needs causal */
+    const int* prefix_len; /* [n_seqs] or NULL */
+    int prefix_both_ways;
+    const int* key_begin;  /* [rows] or NULL */
+    const int* key_end;    /* [rows] or NULL */
+} uocr_hip_attention_opts;
+
+/* Workspace bytes of the two attention calls, for up to `rows` query rows (0 and a message in
+ * uocr_hip_last_error() if the arguments are refused). Grows with the rows of calls that are
+ * split (few rows) and stays under about 160 MB. Calls that overlap in time need a workspace each, two
+ * captured graphs that may run at the same time too. Contents need no setting up. */
+size_t uocr_hip_paged_attention_workspace_size(const uocr_hip_paged_cache* cache, int heads, int rows);
+
+/* Attention of one new token per sequence, its K and V already in the cache: row b of q and out
+ * [batch, heads, head_dim] is position kv_len[s] - 1 of sequence s = d_seqs[b] (b if d_seqs
+ * is NULL); kv_len and prefix_len are indexed by s. A row whose s is not in [0, n_seqs) is padding: its
+ * out is left as it was. max_kv_len bounds kv_len for the choice of the split only
+ * (0: the table's room); results are right, if slower, for longer ones. q has the
+ * cache's type, out that or f32. A row that sees a key whose page is not in [0, n_pages), or whose
+ * kv_len exceeds the table's room, gives NaN; kv_len <= 0 gives zeros. f32 throughout for f32
+ * caches; else f32 scores, statistics and sums of exact products, the
+ * probabilities held in two halves of the cache's type (16 bits of significand or more). The order of
+ * summation depends on sizes only: equal calls give equal bits. out may be q where types agree. */
+int uocr_hip_paged_attention_decode(const uocr_hip_paged_cache* cache, const uocr_hip_attention_opts* opts,
+                                    const uocr_hip_rows* q, int batch, const int* d_seqs, const int* d_kv_len,
+                                    int max_kv_len, const uocr_hip_rows* out, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
+/* Attention of many rows: rows d_q_start[b] .. d_q_start[b + 1] - 1 of q and out
+ * [rows, heads, head_dim] are the last positions of sequence s = d_seqs[b] (b if NULL), whose K and V are
+ * in the cache already: row i of n is position kv_len[s] - n + i. d_q_start has batch + 1 entries, not
+ * falling; rows outside all of them, and rows of an s not in [0, n_seqs), are left as they were. Rows before position 0 (more
+ * rows than kv_len) give zeros. The rest as for the decode call, except that for bf16 and f16 the
+ * probabilities are rounded to that type (relative 2^-9, 2^-12) before they meet V. */
+int uocr_hip_paged_attention_prefill(const uocr_hip_paged_cache* cache, const uocr_hip_attention_opts* opts,
+                                     const uocr_hip_rows* q, int rows, int batch, const int* d_q_start,
+                                     const int* d_seqs, const int* d_kv_len, int max_kv_len, const uocr_hip_rows* out,
+                                     void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

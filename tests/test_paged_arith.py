@@ -1,0 +1,121 @@
+"""CPU check of paged.hpp: what a query row sees, the tiles that walk it, where rows lie in the
+pages (bad entries included), division by the page size, and the split's workspace."""
+import os
+import subprocess
+
+import pytest
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "unlimited-ocr.cpp_amd", "csrc")
+MAIN = r"""
+#include "paged.hpp"
+#include <cstdio>
+#include <cstdlib>
+#include <vector>
+using namespace uocr_hip;
+#define CHECK(x) do { if (!(x)) { printf("line %d: %s\n", __LINE__, #x); return 1; } } while (0)
+
+static int spans() {
+    const int M = 2147483647;
+    for (int causal = 0; causal < 2; ++causal)
+    for (int both = 0; both < 2; ++both)
+    for (int window : {0, 1, 2, 5, 9, M}) {
+        if (window && !causal) continue;
+        for (int len = 0; len < 12; ++len)
+        for (int pos = -2; pos < len; ++pos)
+        for (int prefix : {-1, 0, 1, 3, 7, 11, 20, M})
+        for (int begin : {-M - 1, -1, 0, 2, 6, 20, M})
+        for (int end : {-M - 1, 0, 1, 4, 9, 12, M}) {
+            const Span s = row_span(causal, window, both, pos, len, prefix, begin, end);
+            int n = 0;
+            for (int j = 0; j < len; ++j) {
+                bool seen = !causal || j <= pos;
+                if (window) seen = seen && (long long)j > (long long)pos - window;
+                seen = seen || (j < prefix && (both || !causal || j <= pos));
+                seen = seen && j >= begin && j < end;
+                n += seen;
+                CHECK(s.has(j) == seen);
+            }
+            CHECK(s.count() == n && s.b0 <= s.e0 && s.e0 <= s.b1 && s.b1 <= s.e1);
+            if (n) CHECK((s.b0 == s.e0 || (s.b0 >= 0 && s.e0 <= len)) && (s.b1 == s.e1 || (s.b1 >= 0 && s.e1 <= len)));
+            // every seen key in exactly one tile of its interval, no tile without one
+            const TileWalk w = tile_walk<4>(s);
+            int found = 0;
+            for (int t = 0; t < w.count(); ++t) {
+                const bool first = t < w.n0;
+                const int base = (first ? w.t0 + t : w.t1 + t - w.n0) * 4, b = first ? s.b0 : s.b1, e = first ? s.e0 : s.e1;
+                int here = 0;
+                for (int j = base; j < base + 4; ++j) here += j >= b && j < e;
+                CHECK(here > 0);
+                found += here;
+            }
+            CHECK(found == n);
+        }
+    }
+    // the far end of int
+    const Span s = row_span(1, 100, 0, M - 1, M, 50, 0, M);
+    CHECK(s.b0 == 0 && s.e0 == 50 && s.b1 == M - 100 && s.e1 == M);
+    CHECK(tile_walk<32>(s).count() == 2 + (M - 1) / 32 - (M - 100) / 32 + 1);
+    return 0;
+}
+
+static int places() {
+    for (uint32_t d : {1u, 2u, 3u, 5u, 7u, 16u, 24u, 48u, 100u, 255u, 256u, 1000003u, 1u << 30}) {
+        const FastDiv f = fast_div(d);
+        for (uint64_t n = 0; n < 3000; ++n) CHECK(f.div((uint32_t)n) == n / d);
+        for (uint64_t k = 1; k * d < (1ull << 31); k += 1 + k / 3)
+            for (long long n = (long long)(k * d) - 2; n < (long long)(k * d) + 2; ++n)
+                if (n >= 0 && n < (1ll << 31)) CHECK(f.div((uint32_t)n) == n / d);
+        for (long long n = (1ll << 31) - 3; n < (1ll << 31); ++n) CHECK(f.div((uint32_t)n) == n / d);
+    }
+    const int table[8] = {3, 0, -1, 5, 2, 4, 2147483647, 1};
+    PagedCache c{};
+    c.table = table;
+    c.page_bytes = 3ll << 32;
+    c.row_bytes = 1000;
+    c.table_stride = 4;
+    c.n_pages = 5;
+    c.n_seqs = 2;
+    c.max_pages = 4;
+    c.ps = fast_div(6);
+    CHECK(c.capacity() == 24);
+    for (int s = 0; s < 2; ++s)
+        for (int j = 0; j < 24; ++j) {
+            const int page = table[s * 4 + j / 6];
+            const long long want = page >= 0 && page < 5 ? page * (3ll << 32) + j % 6 * 1000 : -1;
+            CHECK(c.offset(s, j) == want);
+        }
+    c.max_pages = 2147483647;
+    CHECK(c.capacity() == 6ll * 2147483647);
+    return 0;
+}
+
+static int splits() {
+    for (int kv : {1, 2, 8, 10, 40})
+        for (int g : {1, 4, 7, 16, 17, 33})
+            for (long long rows : {1, 2, 3, 9, 33, 100, 257, 1000, 2049, 100000})
+                for (long long r = 1; r <= rows; r += 1 + r / 5)
+                    for (long long tiles : {1, 3, 4, 5, 100, 1000, 70000000}) {
+                        const int n = paged_splits(r * kv * ((g + 15) / 16), tiles);
+                        CHECK(n >= 1 && n <= kPagedMaxSplits && (n == 1 || 4ll * (n - 1) < tiles));
+                        if (n > 1) CHECK((unsigned long long)r * kv * g * n <= paged_workspace_records(rows, kv * g, kv));
+                    }
+    return 0;
+}
+
+int main(int, char** v) { return v[1][0] == 's' ? spans() : v[1][0] == 'p' ? places() : splits(); }
+"""
+
+
+@pytest.fixture(scope="module")
+def run(tmp_path_factory):
+    d = tmp_path_factory.mktemp("paged")
+    (d / "m.cpp").write_text(MAIN)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-fsanitize=undefined", "-fno-sanitize-recover=all", "-I", CSRC,
+                    str(d / "m.cpp"), "-o", str(d / "m")], check=True)
+    return lambda what: subprocess.run([d / "m", what], capture_output=True, text=True)
+
+
+@pytest.mark.parametrize("what", ["spans", "places", "workspace"])
+def test_arithmetic(run, what):
+    r = run(what)
+    assert r.returncode == 0, r.stdout + r.stderr

@@ -1,0 +1,131 @@
+// Paged key-value cache: places of rows in the pages and the keys that a query
+// row sees, shared by the kernels (rope.hip, paged_decode.hip,
+// paged_prefill.hpp), their launchers and a host-side check.
+#pragma once
+
+#include <stdint.h>
+
+namespace uocr_hip {
+
+#ifdef __HIP__
+#define UOCR_HD __host__ __device__
+#else
+#define UOCR_HD
+#endif
+
+constexpr int kPagedTarget = 2048;    // workgroups that a split call aims at
+constexpr int kPagedMaxSplits = 128;
+
+// n / d for 0 <= n < 2^31 by a multiplication: with s = ceil(log2 d) and
+// mul = floor(2^(31+s) / d) + 1, the excess mul * d - 2^(31+s) is at most d <= 2^s,
+// so n * mul / 2^(31+s) is n / d plus less than 1 / d.
+struct FastDiv {
+    uint32_t d, mul, shift;
+    UOCR_HD uint32_t div(uint32_t n) const { return (uint32_t)(((uint64_t)n * mul) >> shift); }
+};
+inline FastDiv fast_div(uint32_t d) {
+    uint32_t s = 0;
+    while ((1ull << s) < d) ++s;
+    return FastDiv{d, (uint32_t)((1ull << (31 + s)) / d + 1), 31 + s};
+}
+
+// The cache as the kernels see it; strides in bytes.
+struct PagedCache {
+    char* k;
+    char* v;
+    const int* table;  // [n_seqs][max_pages], rows table_stride apart
+    long long page_bytes, row_bytes, head_bytes, table_stride;
+    int n_pages, n_seqs, max_pages;
+    FastDiv ps;  // page size
+
+    // rows that the table has room for
+    UOCR_HD long long capacity() const { return (long long)max_pages * ps.d; }
+    // Byte offset of row `pos` of sequence `seq` (both in range: pos < capacity);
+    // -1 where the table names no page of the cache.
+    UOCR_HD long long offset(int seq, int pos) const {
+        const uint32_t t = ps.div((uint32_t)pos);
+        const int page = table[seq * table_stride + t];
+        if ((uint32_t)page >= (uint32_t)n_pages) return -1;
+        return page * page_bytes + (long long)((uint32_t)pos - t * ps.d) * row_bytes;
+    }
+};
+
+// What a query row sees: keys [b0, e0) and [b1, e1), e0 <= b1, either may be empty.
+struct Span {
+    int b0, e0, b1, e1;
+    UOCR_HD bool has(int j) const { return (j >= b0 && j < e0) || (j >= b1 && j < e1); }
+    UOCR_HD int count() const { return (e0 - b0) + (e1 - b1); }
+};
+
+struct MaskArgs {
+    int causal, window, both_ways;  // window 0: none
+    const int* prefix_len;          // [n_seqs] or null
+    const int* key_begin;           // [rows] or null
+    const int* key_end;             // [rows] or null
+};
+
+UOCR_HD inline int imin(int a, int b) { return a < b ? a : b; }
+UOCR_HD inline int imax(int a, int b) { return a > b ? a : b; }
+
+// Row at position `pos` of a sequence of `len` keys, `prefix` of them its prefix, that sees
+// keys [begin, end) at most: key j with j <= pos and j > pos - window (one token has
+// causal set too), or j < prefix (and j <= pos unless the prefix is seen both ways).
+UOCR_HD inline Span row_span(int causal, int window, int both_ways, int pos, int len, int prefix, int begin, int end) {
+    const int hi = causal ? imin(len, pos + 1) : len;          // pos < len <= 2^31 - 1
+    const int lo = window && pos >= window ? pos - window + 1 : 0;
+    const int first = imin(both_ways ? len : hi, prefix);      // the prefix's keys are [0, first)
+    begin = imax(begin, 0);
+    end = imin(end, len);
+    Span s;
+    s.b0 = begin;
+    s.e0 = imax(begin, imin(first, end));
+    s.b1 = imax(imax(lo, s.e0), begin);
+    s.e1 = imax(s.b1, imin(hi, end));
+    // one interval where they touch
+    if (s.b1 == s.e0) {
+        s.e0 = s.e1;
+        s.b1 = s.e1;
+    } else if (s.e0 == s.b0) {
+        s.b0 = s.e0 = s.b1;
+    }
+    return s;
+}
+
+// A row's span as tiles of W keys on W-aligned positions: the first tile that
+// holds a key of each interval, and how many there are. Neighbouring intervals may share a
+// tile; it is walked once for each, with that interval's keys.
+struct TileWalk {
+    int t0, n0, t1, n1;
+    UOCR_HD int count() const { return n0 + n1; }
+};
+template <int W>
+UOCR_HD inline TileWalk tile_walk(const Span& s) {
+    TileWalk w;
+    w.t0 = s.b0 / W;
+    w.n0 = s.e0 > s.b0 ? (s.e0 - 1) / W - w.t0 + 1 : 0;
+    w.t1 = s.b1 / W;
+    w.n1 = s.e1 > s.b1 ? (s.e1 - 1) / W - w.t1 + 1 : 0;
+    return w;
+}
+
+// Splits of a decode call of `units` (sequence, KV head, 16 query heads) with
+// `tiles` tiles of keys at most: enough workgroups for the chip, each of its
+// 4 waves with a tile at least.
+inline int paged_splits(long long units, long long tiles) {
+    const long long want = (kPagedTarget + units - 1) / units, most = (tiles + 3) / 4;
+    long long n = want < most ? want : most;
+    if (n > kPagedMaxSplits) n = kPagedMaxSplits;
+    return n < 1 ? 1 : (int)n;
+}
+
+// Partial results (row, head, split) that a call of up to `rows` rows may hold: with one row per
+// unit of up to 16 heads, units * splits stays below kPagedTarget + units, and
+// calls of kPagedTarget units are not split.
+inline unsigned long long paged_workspace_records(long long rows, int heads, int kv_heads) {
+    const int blocks = (heads / kv_heads + 15) / 16;
+    const long long full = kPagedTarget / ((long long)kv_heads * blocks) + 1;  // rows of a call that is not split
+    const long long n = rows * kPagedMaxSplits, most = full + (rows < full ? rows : full);
+    return (unsigned long long)heads * (n < most ? n : most);
+}
+
+}  // namespace uocr_hip

@@ -15,6 +15,7 @@ EWORKSPACE = -4
 EHIP = -5
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
+DTYPE_F16 = 2
 
 
 class HipError(RuntimeError):
@@ -50,6 +51,29 @@ class LayerDescC(C.Structure):
                 ("shared_gate_w", C.POINTER(DenseMatrixC)), ("shared_up_w", C.POINTER(DenseMatrixC)),
                 ("shared_down_w", C.POINTER(DenseMatrixC)), ("gate_w", C.POINTER(DenseMatrixC)),
                 ("up_w", C.POINTER(DenseMatrixC)), ("down_w", C.POINTER(DenseMatrixC))]
+
+
+class RowsC(C.Structure):
+    """uocr_hip_rows: rows of heads by strides (elements)."""
+
+    _fields_ = [("data", C.c_void_p), ("dtype", C.c_int), ("row_stride", C.c_longlong), ("head_stride", C.c_longlong)]
+
+
+class PagedCacheC(C.Structure):
+    """uocr_hip_paged_cache."""
+
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int), ("n_pages", C.c_int), ("page_size", C.c_int),
+                ("kv_heads", C.c_int), ("head_dim", C.c_int), ("page_stride", C.c_longlong),
+                ("row_stride", C.c_longlong), ("head_stride", C.c_longlong), ("page_table", C.c_void_p),
+                ("n_seqs", C.c_int), ("max_pages", C.c_int), ("table_stride", C.c_longlong)]
+
+
+class AttentionOptsC(C.Structure):
+    """uocr_hip_attention_opts."""
+
+    _fields_ = [("heads", C.c_int), ("scale", C.c_float), ("softcap", C.c_float), ("slopes", C.c_void_p),
+                ("causal", C.c_int), ("window", C.c_int), ("prefix_len", C.c_void_p), ("prefix_both_ways", C.c_int),
+                ("key_begin", C.c_void_p), ("key_end", C.c_void_p)]
 
 
 def lib_path():
@@ -115,6 +139,12 @@ SIGNATURES = {
     "uocr_hip_add_scaled": (C.c_int, [C.c_void_p, C.c_void_p, C.c_float, C.c_int, C.c_void_p]),
     "uocr_hip_scatter_add_scaled": (C.c_int, [C.c_void_p] * 4 + [C.c_int, C.c_int, C.c_void_p]),
     "uocr_hip_gather_rows": (C.c_int, [C.c_void_p] * 3 + [C.c_int, C.c_int, C.c_void_p]),
+    "uocr_hip_rope_frequencies": (C.c_int, [C.c_int, C.c_double, C.c_int, C.c_double, C.c_int, C.c_double, C.c_double, C.c_void_p, C.POINTER(C.c_float)]),
+    "uocr_hip_rope": (C.c_int, [C.c_void_p] * 2 + [C.c_int] * 4 + [C.c_void_p] * 2 + [C.c_int] * 2 + [C.c_float] + [C.c_void_p] * 3),
+    "uocr_hip_rope_append_paged": (C.c_int, [C.c_void_p] * 3 + [C.c_int] * 2 + [C.c_void_p] * 2 + [C.c_int] * 2 + [C.c_float] + [C.c_void_p] * 5),
+    "uocr_hip_paged_attention_workspace_size": (C.c_size_t, [C.c_void_p, C.c_int, C.c_int]),
+    "uocr_hip_paged_attention_decode": (C.c_int, [C.c_void_p] * 3 + [C.c_int] + [C.c_void_p] * 2 + [C.c_int] + [C.c_void_p] * 2 + [C.c_size_t, C.c_void_p]),
+    "uocr_hip_paged_attention_prefill": (C.c_int, [C.c_void_p] * 3 + [C.c_int] * 2 + [C.c_void_p] * 3 + [C.c_int] + [C.c_void_p] * 2 + [C.c_size_t, C.c_void_p]),
     "uocr_hip_moe_router_topk": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int,
                                             C.c_float, C.c_int, C.c_void_p, C.c_void_p,
                                             C.c_void_p, C.c_void_p, C.c_void_p, C.c_int,
