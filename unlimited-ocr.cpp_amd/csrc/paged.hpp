@@ -14,6 +14,7 @@ namespace uocr_hip {
 #endif
 
 constexpr int kPagedTarget = 2048;    // workgroups that a split call aims at
+constexpr int kPagedPrefillTarget = 512;
 constexpr int kPagedMaxSplits = 128;
 
 // n / d for 0 <= n < 2^31 by a multiplication: with s = ceil(log2 d) and
@@ -118,14 +119,26 @@ inline int paged_splits(long long units, long long tiles) {
     return n < 1 ? 1 : (int)n;
 }
 
-// Partial results (row, head, split) that a call of up to `rows` rows may hold: with one row per
-// unit of up to 16 heads, units * splits stays below kPagedTarget + units, and
-// calls of kPagedTarget units are not split.
+// Splits of a prefill call of `units` (tile, KV head) workgroups: where they leave most of
+// the chip idle, each split with 4 tiles of keys at least.
+inline int paged_prefill_splits(long long units, long long tiles) {
+    const long long want = kPagedPrefillTarget / units, most = tiles / 4;
+    long long n = want < most ? want : most;
+    if (n > kPagedMaxSplits) n = kPagedMaxSplits;
+    return n < 1 ? 1 : (int)n;
+}
+
+// Partial results (row, head, split) that a call of up to `rows` rows may hold.
+// Decode: one row per unit of up to 16 heads; units * splits stays below kPagedTarget + units, and
+// calls of kPagedTarget units are not split. Prefill: a unit is 128 (row, head) pairs of a KV head at most, and
+// units * splits stays below kPagedPrefillTarget.
 inline unsigned long long paged_workspace_records(long long rows, int heads, int kv_heads) {
-    const int blocks = (heads / kv_heads + 15) / 16;
-    const long long full = kPagedTarget / ((long long)kv_heads * blocks) + 1;  // rows of a call that is not split
-    const long long n = rows * kPagedMaxSplits, most = full + (rows < full ? rows : full);
-    return (unsigned long long)heads * (n < most ? n : most);
+    const long long group = heads / kv_heads, blocks = (group + 15) / 16;
+    const long long full = kPagedTarget / (kv_heads * blocks) + 1;  // rows of a call that is not split
+    const long long any = rows * heads * kPagedMaxSplits;
+    long long decode = heads * (full + (rows < full ? rows : full)), prefill = 128ll * kPagedPrefillTarget;
+    const long long most = decode > prefill ? decode : prefill;
+    return (unsigned long long)(any < most ? any : most);
 }
 
 }  // namespace uocr_hip

@@ -1,0 +1,504 @@
+// Attention of many query rows over a paged KV cache, tiled on MFMA
+// (instantiated per type in paged_prefill_{bf16,f16,f32}.hip).
+//
+// out = softmax(s) V row by row, s = scale q.k with cap, bias and mask; one pass over the
+// keys with a running maximum and sum per row. Bound by the matrix cores: 4 head_dim
+// operations per visible pair and head.
+//
+// A workgroup of 4 waves takes 128 query rows of one KV head: the `group` query heads that
+// share it side by side for each token, so that K and V tiles serve all of them. Tiles of
+// 64 keys (32 for f32) go through registers into LDS, the next one in flight during the
+// current one's products; registers (and not a direct load) because pages may
+// start anywhere and rows are padded. Each wave has 32 rows:
+//   * S^T = K Q^T on v_mfma_f32_32x32x16: lane (i, h) = (lane % 32, lane / 32) holds row i's
+//     scores of keys 8 (r / 4) + 4 h + r % 4, so a row's maximum and sum need one exchange between
+//     the halves of the wave, and ...
+//   * ... O^T = V^T P^T takes the probabilities where they are: a 16-key step's slots (h, e) are
+//     keys 4 h + e and 4 h + 8 + e - 4. V's transposed operand comes from LDS by
+//     ds_read_b64_tr_b16 (4 keys x 16 dims per 16 lanes); f32 reads it directly.
+// LDS rows are padded so that these reads cover all banks: K rows to an odd multiple
+// of 16 bytes, V rows to 64 bytes more or less than a multiple of 256 (f32: 32 bytes more).
+// The running maximum is raised only where a score passes it by 2^8 (probabilities up to 256 are as
+// exact as those up to 1), so sums are rarely rescaled.
+// Rows whose result is not finite, or that saw a key without a page, are done again by row_attention:
+// NaN and infinities of keys that only other rows of the tile see do not reach them.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include "launch.hpp"
+#include "paged_device.hpp"
+#include "paged_host.hpp"
+#include "xcd_order.hpp"
+
+namespace uocr_hip {
+
+constexpr int kPreRows = 128;  // packed query rows per workgroup
+constexpr int kPreWaves = 4;
+template <typename T>
+constexpr int kPreKeys = sizeof(T) == 4 ? 32 : 64;  // keys per tile
+
+template <typename T, int DP>
+struct PreShape {
+    static constexpr int ES = sizeof(T);
+    static constexpr int KSTR = DP * ES + 16;
+    static constexpr int VPAD = ES == 4 ? 32 : (DP * 2 % 256 == 64 || DP * 2 % 256 == 192) ? 0 : 64;
+    static constexpr int VSTR = DP * ES + VPAD;
+    static constexpr int BYTES = kPreKeys<T> * (KSTR + VSTR);  // one buffer
+};
+
+// Row range of sequence entry b in [0, rows]
+__device__ __forceinline__ int pre_start(const PagedAttnArgs& a, int b) { return imin(imax(a.q_start[b], 0), a.rows); }
+
+// Entry b and tile within it of tile index t (tiles of entry after entry); -1: none
+__device__ __forceinline__ int pre_find(const PagedAttnArgs& a, int t, int& tile) {
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+        const int b = b0 + lane;
+        int n = 0;
+        if (b < a.batch) n = (imax(pre_start(a, b + 1) - pre_start(a, b), 0) * a.group + kPreRows - 1) / kPreRows;
+        int sum = n;
+#pragma unroll
+        for (int x = 1; x < 64; x *= 2) {
+            const int y = __shfl_up(sum, x, 64);
+            if (lane >= x) sum += y;
+        }
+        const uint64_t hit = __ballot(before + sum > t);
+        if (hit) {
+            const int src = __builtin_ctzll(hit);
+            tile = t - before - (__shfl(sum, src, 64) - __shfl(n, src, 64));
+            return b0 + src;
+        }
+        before += __shfl(sum, 63, 64);
+    }
+    return -1;
+}
+
+__device__ __forceinline__ int wave_min(int v) {
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) v = imin(v, __shfl_xor(v, x, 64));
+    return v;
+}
+__device__ __forceinline__ int wave_max(int v) { return -wave_min(-v); }
+
+// max over the two halves of a wave
+__device__ __forceinline__ float half_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// bits [b, e) of a 64-bit word, any ints
+__device__ __forceinline__ uint64_t bits(int b, int e) {
+    b = imin(imax(b, 0), 64);
+    e = imin(imax(e, 0), 64);
+    if (b >= e) return 0;
+    return (e == 64 ? ~0ull : (1ull << e) - 1) & ~(b == 64 ? ~0ull : (1ull << b) - 1);
+}
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ s16x4 lds_tr(const char* p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) s16x4*)(__attribute__((address_space(3))) void*)(void*)p);
+}
+
+template <typename T, int DP, bool CAP, bool BIAS>
+__global__ __launch_bounds__(kPreWaves * 64, DP > 128 ? 1 : 2) void paged_prefill_kernel(PagedAttnArgs a) {
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int ES = sizeof(T), BN = kPreKeys<T>, KB = BN / 32, CH = DP * ES / 16, NL = BN * CH / (kPreWaves * 64);
+    static_assert(BN * CH % (kPreWaves * 64) == 0, "whole 16-byte units per thread");
+    constexpr int KSTR = PreShape<T, DP>::KSTR, VSTR = PreShape<T, DP>::VSTR, BUF = PreShape<T, DP>::BYTES;
+    constexpr int NF = F32 ? DP / 8 : DP / 16;  // 16-byte pieces of a query row per lane
+    constexpr int DB = DP / 32;
+    typedef typename Vec8<T>::type vec_t;
+    extern __shared__ __attribute__((aligned(16))) char s_buf[];  // two buffers: K rows, then V rows
+    __shared__ int s_range[kPreWaves][4];
+    __shared__ int s_lost;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 31, h = lane >> 5;
+    // Items (KV head, tile), an eighth in order per XCD: a KV head's tiles share
+    // its K and V in one L2. Last tiles first: they see the most keys under a causal mask.
+    const int items = a.n_tiles * a.kv_heads, per = gridDim.x / a.n_splits;
+    const int split = blockIdx.x / per, blk = blockIdx.x % per, xcd = blk % kXcds;
+    const int first = xcd_first_item(xcd, items), item = first + blk / kXcds;
+    if (item >= xcd_first_item(xcd + 1, items)) return;
+    const int kvh = item / a.n_tiles;
+    int tile;
+    const int entry = pre_find(a, a.n_tiles - 1 - item % a.n_tiles, tile);
+    if (entry < 0) return;
+    const int seq = a.seqs ? a.seqs[entry] : entry;
+    if ((uint32_t)seq >= (uint32_t)a.c.n_seqs) return;
+    const int start = pre_start(a, entry), n = imax(pre_start(a, entry + 1) - start, 0);
+    const int kv = a.kv_len[seq];
+    const bool gone = kv > a.c.capacity();  // more keys than the table has room for
+    const int len = gone ? 0 : imax(kv, 0);
+
+    // this lane's query row
+    const int packed = tile * kPreRows + wave * 32 + i;
+    const bool live = packed < n * a.group;
+    const int token = packed / a.group, row = start + imin(token, n - 1), head = kvh * a.group + packed % a.group;
+    const int pos = len - n + token;
+    Span span{0, 0, 0, 0};
+    if (live)
+        span = row_span(a.mask.causal, a.mask.window, a.mask.both_ways, pos, len, a.mask.prefix_len ? a.mask.prefix_len[seq] : 0,
+                        a.mask.key_begin ? a.mask.key_begin[row] : 0, a.mask.key_end ? a.mask.key_end[row] : len);
+    // keys that some row sees: two ranges
+    {
+        constexpr int kFar = 0x7fffffff;
+        const bool in0 = span.e0 > span.b0, in1 = span.e1 > span.b1;
+        const int r0 = wave_min(in0 ? span.b0 : kFar), r1 = wave_max(in0 ? span.e0 : 0);
+        const int r2 = wave_min(in1 ? span.b1 : kFar), r3 = wave_max(in1 ? span.e1 : 0);
+        if (lane == 0) {
+            s_range[wave][0] = r0;
+            s_range[wave][1] = r1;
+            s_range[wave][2] = r2;
+            s_range[wave][3] = r3;
+        }
+        if (tid == 0) s_lost = 0;
+    }
+    __syncthreads();
+    int lo0 = s_range[0][0], hi0 = s_range[0][1], lo1 = s_range[0][2], hi1 = s_range[0][3];
+#pragma unroll
+    for (int w = 1; w < kPreWaves; ++w) {
+        lo0 = imin(lo0, s_range[w][0]);
+        hi0 = imax(hi0, s_range[w][1]);
+        lo1 = imin(lo1, s_range[w][2]);
+        hi1 = imax(hi1, s_range[w][3]);
+    }
+    // as tiles; one range where a tile would be in both
+    int t0 = hi0 ? lo0 / BN : 0, n0 = hi0 ? (hi0 - 1) / BN + 1 - t0 : 0;
+    int t1 = hi1 ? lo1 / BN : 0, n1 = hi1 ? (hi1 - 1) / BN + 1 - t1 : 0;
+    if (n0 && n1 && t0 < t1 + n1 && t1 < t0 + n0) {
+        const int e = imax(t0 + n0, t1 + n1);
+        t0 = imin(t0, t1);
+        n0 = e - t0;
+        n1 = 0;
+        lo0 = imin(lo0, lo1);
+        hi0 = imax(hi0, hi1);
+    }
+    const int tiles = n0 + n1, share = (tiles + a.n_splits - 1) / a.n_splits;
+    const int t_begin = imin(split * share, tiles), t_end = imin(t_begin + share, tiles);
+
+    // query operand: dims 16 f + 8 h .. + 7 (f32: 8 f + 4 h .. + 3) of row i
+    vec_t q[NF];
+    {
+        const char* qp = a.q.p + row * a.q.row_bytes + head * a.q.head_bytes;
+        // a negative scale is moved into q: the maximum is taken before the scale
+        const uint32_t flip = a.sc.scale < 0.0f ? (F32 ? 0x80000000u : 0x80008000u) : 0u;
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+            const int d = (2 * f + h) * (16 / ES);
+            const bool in = live && d < a.head_dim;
+            u32x4 w = {0, 0, 0, 0};
+            if (in) w = *reinterpret_cast<const u32x4*>(qp + d * ES);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] ^= flip;
+            q[f] = as_vec<vec_t>(w);
+        }
+    }
+    PagedScores sc = a.sc;
+    sc.scale = fabsf(sc.scale);
+    const float scale2 = sc.scale * kLog2e;
+    float slope2 = 0.0f;
+    if constexpr (BIAS) slope2 = a.sc.slopes[head] * kLog2e;
+
+    // tile t of the block's ranges: K and V to registers, then to LDS
+    const char* kbase = a.c.k + kvh * a.c.head_bytes;
+    const char* vbase = a.c.v + kvh * a.c.head_bytes;
+    u32x4 kw[NL], vw[NL];
+    auto tile_base = [&](int t) { return (t < n0 ? t0 + t : t1 + t - n0) * BN; };
+    auto place = [&](int t) {  // of key `lane` (mod BN); keys outside the range: those at its ends
+        const int lo = t < n0 ? lo0 : lo1, hi = t < n0 ? hi0 : hi1;
+        long long off = a.c.offset(seq, imin(imax(tile_base(t) + (lane & (BN - 1)), lo), hi - 1));
+        if (off < 0) {
+            s_lost = 1;
+            off = 0;
+        }
+        return off;
+    };
+    auto load = [&](long long off) {
+#pragma unroll
+        for (int e = 0; e < NL; ++e) {
+            const int u = e * (kPreWaves * 64) + tid, r = u / CH, c = u % CH;
+            const long long at = shfl64(off, r) + c * 16;
+            kw[e] = vw[e] = u32x4{0, 0, 0, 0};
+            if (c * (16 / ES) < a.head_dim) {
+                kw[e] = *reinterpret_cast<const u32x4*>(kbase + at);
+                vw[e] = *reinterpret_cast<const u32x4*>(vbase + at);
+            }
+        }
+    };
+    auto store = [&](char* buf) {
+#pragma unroll
+        for (int e = 0; e < NL; ++e) {
+            const int u = e * (kPreWaves * 64) + tid, r = u / CH, c = u % CH;
+            *reinterpret_cast<u32x4*>(buf + r * KSTR + c * 16) = kw[e];
+            *reinterpret_cast<u32x4*>(buf + BN * KSTR + r * VSTR + c * 16) = vw[e];
+        }
+    };
+
+    float m = -INFINITY, l = 0.0f;  // of row i (l: over this lane's keys), in log 2
+    f32x16 o[DB] = {};
+    if (t_begin < t_end) {
+        load(place(t_begin));
+        long long next = t_begin + 1 < t_end ? place(t_begin + 1) : 0;
+        store(s_buf);
+        for (int t = t_begin; t < t_end; ++t) {
+            __syncthreads();
+            const char* buf = s_buf + ((t - t_begin) & 1) * BUF;
+            if (t + 1 < t_end) load(next);
+            if (t + 2 < t_end) next = place(t + 2);
+            const int base = tile_base(t);
+            const uint64_t seen = bits(span.b0 - base, span.e0 - base) | bits(span.b1 - base, span.e1 - base);
+            constexpr uint64_t kAll = BN == 64 ? ~0ull : (1ull << BN) - 1;
+            if (__any((seen & kAll) != 0)) {
+                f32x16 s[KB];
+#pragma unroll
+                for (int b = 0; b < KB; ++b) {
+                    s[b] = f32x16{};
+                    const char* kp = buf + (b * 32 + i) * KSTR + h * 16;
+#pragma unroll
+                    for (int f = 0; f < NF; ++f) {
+                        const vec_t k = *reinterpret_cast<const vec_t*>(kp + f * 32);
+                        if constexpr (F32) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) s[b] = mfma_32x32x2(k[e], q[f][e], s[b]);
+                        } else {
+                            s[b] = mfma_32x32x16(k, q[f], s[b]);
+                        }
+                    }
+                }
+                const bool whole = __all((seen & kAll) == kAll);
+                if constexpr (CAP || BIAS) {
+                    const int dist0 = pos - base - 4 * h;
+#pragma unroll
+                    for (int b = 0; b < KB; ++b)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            s[b][r] = score2<CAP, BIAS, F32>(s[b][r], sc, slope2, dist0 - (b * 32 + 8 * (r >> 2) + (r & 3)));
+                }
+                constexpr bool kScaled = CAP || BIAS;
+                if (!whole) {
+                    const uint64_t mine = seen >> (4 * h);
+#pragma unroll
+                    for (int b = 0; b < KB; ++b)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            s[b][r] = (uint32_t)(mine >> (32 * b)) >> (8 * (r >> 2) + (r & 3)) & 1 ? s[b][r] : -INFINITY;
+                }
+                float top = -INFINITY;
+#pragma unroll
+                for (int b = 0; b < KB; ++b)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
+                top = half_max(top);
+                if constexpr (!kScaled) top *= scale2;
+                if (__any(top > m + 8.0f)) {
+                    const float up = fmaxf(m, top), ref = up == -INFINITY ? 0.0f : up;
+                    const float alpha = __builtin_amdgcn_exp2f(m - ref);
+                    m = up;
+                    l *= alpha;
+#pragma unroll
+                    for (int d = 0; d < DB; ++d)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+                }
+                const float ref = m == -INFINITY ? 0.0f : m;
+                float sum[4] = {};
+#pragma unroll
+                for (int b = 0; b < KB; ++b)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        s[b][r] = __builtin_amdgcn_exp2f(kScaled ? s[b][r] - ref : fmaf(s[b][r], scale2, -ref));
+                        sum[r & 3] += s[b][r];
+                    }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                const char* vp = buf + BN * KSTR;
+                if constexpr (F32) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+#pragma unroll
+                        for (int d = 0; d < DB; ++d)
+                            o[d] = mfma_32x32x2(*reinterpret_cast<const float*>(vp + (8 * (r >> 2) + (r & 3) + 4 * h) * VSTR + (d * 32 + i) * 4),
+                                                s[0][r], o[d]);
+                } else {
+                    vp += (4 * h + (lane >> 2 & 3)) * VSTR + (lane >> 4 & 1) * 32 + (lane & 3) * 8;
+#pragma unroll
+                    for (int st = 0; st < KB * 2; ++st) {
+                        vec_t p;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) p[e] = (T)s[st >> 1][8 * (st & 1) + e];
+#pragma unroll
+                        for (int d = 0; d < DB; ++d) {
+                            s16x4 v[2];
+                            v[0] = lds_tr(vp + st * 16 * VSTR + d * 64);
+                            v[1] = lds_tr(vp + (st * 16 + 8) * VSTR + d * 64);
+                            vec_t vv;
+                            __builtin_memcpy(&vv, v, 16);
+                            o[d] = mfma_32x32x16(vv, p, o[d]);
+                        }
+                    }
+                }
+            }
+            if (t + 1 < t_end) store(s_buf + ((t + 1 - t_begin) & 1) * BUF);
+        }
+    }
+    __syncthreads();
+    l += __shfl_xor(l, 32, 64);
+    if (a.n_splits > 1) {
+        if (live) {
+            const size_t rec = ((size_t)row * a.heads + head) * a.n_splits + split;
+            if (h == 0) {
+                a.part_ml[2 * rec] = m;
+                a.part_ml[2 * rec + 1] = s_lost ? NAN : l;  // (the join does such a row again)
+            }
+            if (m != -INFINITY || l != 0.0f) {
+                float* p = a.part + rec * a.head_dim;
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int r = 0; r < 16; r += 4) {
+                        const int d0 = d * 32 + 2 * r + 4 * h;
+                        if (d0 < a.head_dim)
+                            *reinterpret_cast<f32x4*>(p + d0) = f32x4{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
+                    }
+            }
+        }
+        return;
+    }
+    const float inv = 1.0f / l;
+    bool bad = s_lost || !(l > 0.0f && l < INFINITY);
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            o[d][r] *= inv;
+            bad |= !(fabsf(o[d][r]) < INFINITY);
+        }
+    if (span.count() == 0) {
+        bad = false;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[d][r] = gone ? NAN : 0.0f;
+    }
+    uint64_t again = __ballot(bad && live);
+    again = (again | again >> 32) & 0xffffffffu;
+    if (live && !(again >> i & 1)) {
+        char* op = a.out.p + row * a.out.row_bytes + head * a.out.head_bytes;
+        const int es = a.out_f32 ? 4 : ES;
+        const bool wide = (((uintptr_t)a.out.p | a.out.row_bytes | a.out.head_bytes) & (4 * es - 1)) == 0;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int d0 = d * 32 + 2 * r + 4 * h;
+                if (d0 >= a.head_dim) continue;
+                const f32x4 v = {o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
+                if (F32 || a.out_f32) {
+                    float* p = reinterpret_cast<float*>(op) + d0;
+                    if (wide) *reinterpret_cast<f32x4*>(p) = v;
+                    else
+                        for (int e = 0; e < 4; ++e) p[e] = v[e];
+                } else {
+                    T* p = reinterpret_cast<T*>(op) + d0;
+                    T t[4] = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+                    if (wide) __builtin_memcpy(__builtin_assume_aligned(p, 8), t, 8);
+                    else
+                        for (int e = 0; e < 4; ++e) p[e] = t[e];
+                }
+            }
+    }
+    for (; again; again &= again - 1) {
+        const int src = __builtin_ctzll(again);
+        row_attention<T>(a, seq, __shfl(row, src, 64), __shfl(head, src, 64), __shfl(pos, src, 64), len, gone);
+    }
+}
+
+// Joins the splits of each (row, head), in their order: one wave each.
+template <typename T>
+__global__ __launch_bounds__(256) void paged_prefill_join_kernel(PagedAttnArgs a) {
+    const int lane = threadIdx.x & 63;
+    const long long u = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (u >= (long long)a.rows * a.heads) return;
+    const int row = (int)(u / a.heads), head = (int)(u % a.heads);
+    // the entry whose rows include it
+    int lo = 0, hi = a.batch;
+    while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (a.q_start[mid + 1] > row) hi = mid;
+        else lo = mid + 1;
+    }
+    if (lo >= a.batch || a.q_start[lo] > row) return;
+    const int seq = a.seqs ? a.seqs[lo] : lo;
+    if ((uint32_t)seq >= (uint32_t)a.c.n_seqs) return;
+    const int kv = a.kv_len[seq];
+    const bool gone = kv > a.c.capacity();
+    const int len = gone ? 0 : imax(kv, 0), start = pre_start(a, lo), n = pre_start(a, lo + 1) - start;
+    const size_t rec = (size_t)u * a.n_splits;
+    float M = -INFINITY;
+    for (int s = 0; s < a.n_splits; ++s) M = fmaxf(M, a.part_ml[2 * (rec + s)]);
+    const float ref = M == -INFINITY ? 0.0f : M;
+    float L = 0.0f, o[4] = {};
+    for (int s = 0; s < a.n_splits; ++s) {
+        const float ms = a.part_ml[2 * (rec + s)], ls = a.part_ml[2 * (rec + s) + 1];
+        if (ms == -INFINITY && ls == 0.0f) continue;  // (no sums were written)
+        const float f = __builtin_amdgcn_exp2f(ms - ref);
+        L = fmaf(ls, f, L);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (lane + 64 * e < a.head_dim) o[e] = fmaf(a.part[(rec + s) * a.head_dim + lane + 64 * e], f, o[e]);
+    }
+    bool bad = !(L > 0.0f && L < INFINITY);
+    const float inv = 1.0f / L;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        o[e] *= inv;
+        bad |= !(fabsf(o[e]) < INFINITY) && lane + 64 * e < a.head_dim;
+    }
+    if (__any(bad)) {  // (rows that see nothing, too)
+        row_attention<T>(a, seq, row, head, len - n + (row - start), len, gone);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (lane + 64 * e < a.head_dim) store_out(a, (const T*)nullptr, row, head, lane + 64 * e, o[e]);
+}
+
+template <typename T, int DP>
+int launch_prefill_dp(const PagedAttnArgs& a, dim3 grid, hipStream_t st) {
+    const dim3 block(kPreWaves * 64);
+    const uint32_t lds = 2 * PreShape<T, DP>::BYTES;
+    const bool cap = a.sc.softcap > 0.0f, bias = a.sc.slopes != nullptr;
+    const auto go = [&](auto kernel) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess)
+            return set_error(UOCR_HIP_EHIP, std::string("paged prefill LDS: ") + hipGetErrorString(e));
+        launch_k(kernel, grid, block, lds, st, a);
+        return UOCR_HIP_OK;
+    };
+    if (cap && bias) return go(paged_prefill_kernel<T, DP, true, true>);
+    if (cap) return go(paged_prefill_kernel<T, DP, true, false>);
+    if (bias) return go(paged_prefill_kernel<T, DP, false, true>);
+    return go(paged_prefill_kernel<T, DP, false, false>);
+}
+
+template <typename T>
+int launch_prefill_t(const PagedAttnArgs& a, dim3 grid, hipStream_t st) {
+    int rc;
+    if (a.head_dim <= 64) rc = launch_prefill_dp<T, 64>(a, grid, st);
+    else if (a.head_dim <= 96) rc = launch_prefill_dp<T, 96>(a, grid, st);
+    else if (a.head_dim <= 128) rc = launch_prefill_dp<T, 128>(a, grid, st);
+    else if (a.head_dim <= 192) rc = launch_prefill_dp<T, 192>(a, grid, st);
+    else rc = launch_prefill_dp<T, 256>(a, grid, st);
+    if (rc) return rc;
+    if (a.n_splits > 1)
+        launch_k(paged_prefill_join_kernel<T>, dim3((unsigned)(((long long)a.rows * a.heads + 3) / 4)), dim3(256), 0, st, a);
+    return UOCR_HIP_OK;
+}
+
+int launch_prefill_f32(const PagedAttnArgs& a, dim3 grid, hipStream_t st);
+int launch_prefill_bf16(const PagedAttnArgs& a, dim3 grid, hipStream_t st);
+int launch_prefill_f16(const PagedAttnArgs& a, dim3 grid, hipStream_t st);
+
+}  // namespace uocr_hip
