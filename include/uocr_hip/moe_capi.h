@@ -580,10 +580,13 @@ typedef struct {
 } uocr_hip_attention_opts;
 
 /* Workspace bytes of the two attention calls, for up to `rows` query rows (0 and a message in
- * uocr_hip_last_error() if the arguments are refused). Grows with the rows of calls that are
- * split (few rows) and stays under about 160 MB. Calls that overlap in time need a workspace each, two
- * captured graphs that may run at the same time too. Contents need no setting up. */
+ * uocr_hip_last_error() if the arguments are refused): at most about 160 MB, most of it for calls
+ * with heads of 256. A workspace is set up once, by _workspace_init, before its first call, and again if a call
+ * on it was cut short; calls leave it ready for the next, of any shape that it is large enough for. Calls that
+ * overlap in time need a workspace each, two captured graphs that may run at the same time too. A decode
+ * call on one that was not set up gives NaN. */
 size_t uocr_hip_paged_attention_workspace_size(const uocr_hip_paged_cache* cache, int heads, int rows);
+int uocr_hip_paged_attention_workspace_init(void* workspace, size_t workspace_bytes, void* stream);
 
 /* Attention of one new token per sequence, its K and V already in the cache: row b of q and out
  * [batch, heads, head_dim] is position kv_len[s] - 1 of sequence s = d_seqs[b] (b if d_seqs

@@ -152,7 +152,6 @@ def run_decode(dev, rng, pool, heads, out_dtype=None, seqs=None, spread=1.5, str
     if arg.get("slopes") is not None:
         arg["slopes"] = torch.tensor(arg["slopes"], dtype=torch.float32, device=dev)
     ws = paged().attention_workspace(cache, heads, n)
-    ws.fill_(255)
     paged().attention_decode(qd, cache, pool.kv_len, out, seqs=None if seqs is None else i32(seqs, dev), workspace=ws, **arg)
     for i, b in enumerate(rows):
         if not 0 <= b < len(pool.lens):
@@ -217,6 +216,39 @@ def test_decode_split_f32_large_scores(dev):
     rng = np.random.default_rng(23)
     pool = R.Pool(rng, [2500, 900], 2, 64, 32, "f32", dev, std=3.0)
     run_decode(dev, rng, pool, 2, spread=40.0)
+
+
+@pytest.mark.parametrize("heads,kv_heads,d,lens,hint", [
+    (4, 1, 64, [9000], 0), (32, 2, 128, [2500, 2500, 1, 0, 40], 2500), (3, 3, 96, [1200] * 9, 0), (16, 1, 256, [1500, 700], 0),
+    (18, 1, 64, [800] * 40, 0), (2, 2, 128, [30] * 300, 2000)])
+def test_decode_shares(dev, heads, kv_heads, d, lens, hint):
+    """Many shares of one sequence (joined by a kernel of its own), a few of each, several sequences in one; on one
+    workspace in turn, so that each call leaves it as the next needs it."""
+    rng = np.random.default_rng(len(lens))
+    pool = R.Pool(rng, lens, kv_heads, d, 16, "bf16", dev)
+    first = run_decode(dev, np.random.default_rng(1), pool, heads, max_kv_len=hint)
+    cache = pool.cache()
+    ws = paged().attention_workspace(cache, heads, len(lens))
+    q = rand(np.random.default_rng(1), len(lens), heads + 1, d + 8, std=1.5).to(torch.bfloat16)[:, 1:, :d].contiguous().to(dev)
+    for _ in range(4):
+        out = torch.zeros_like(q)
+        paged().attention_decode(q, cache, pool.kv_len, out, max_kv_len=hint, workspace=ws)
+        assert torch.equal(out, first)
+        few = torch.zeros_like(q[:1])
+        paged().attention_decode(q[:1], cache, pool.kv_len, few, max_kv_len=0, workspace=ws)
+        assert torch.isfinite(few).all()
+
+
+def test_decode_workspace_that_was_not_set_up(dev):
+    """NaN, not something that looks like a result."""
+    rng = np.random.default_rng(3)
+    pool = R.Pool(rng, [2000, 700], 1, 64, 16, "bf16", dev)
+    cache = pool.cache()
+    q = rand(rng, 2, 2, 64).to(torch.bfloat16).to(dev)
+    out = torch.zeros_like(q)
+    ws = torch.zeros_like(paged().attention_workspace(cache, 2, 2))
+    paged().attention_decode(q, cache, pool.kv_len, out, workspace=ws)
+    assert torch.isnan(out).all()
 
 
 def test_decode_padding_and_order(dev):

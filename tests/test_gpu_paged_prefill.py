@@ -34,7 +34,6 @@ def run_prefill(dev, rng, pool, q_rows, heads, out_dtype=None, seqs=None, spread
     if arg.get("slopes") is not None:
         arg["slopes"] = torch.tensor(arg["slopes"], dtype=torch.float32, device=dev)
     ws = paged().attention_workspace(cache, heads, n)
-    ws.fill_(255)
     paged().attention_prefill(qd, cache, i32(starts, dev), pool.kv_len, out, seqs=None if seqs is None else i32(seqs, dev),
                               workspace=ws, **arg)
     res = out.cpu()

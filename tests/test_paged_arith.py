@@ -92,12 +92,22 @@ static int places() {
 static int splits() {
     for (int kv : {1, 2, 8, 10, 40})
         for (int g : {1, 4, 7, 16, 17, 33})
-            for (long long rows : {1, 2, 3, 9, 33, 100, 257, 1000, 2049, 100000})
+            for (long long rows : {1, 2, 3, 9, 33, 100, 257, 1000, 1024, 1025, 100000})
                 for (long long r = 1; r <= rows; r += 1 + r / 5)
-                    for (long long tiles : {1, 3, 4, 5, 100, 1000, 70000000}) {
-                        const int n = paged_splits(r * kv * ((g + 15) / 16), tiles);
-                        CHECK(n >= 1 && n <= kPagedMaxSplits && (n == 1 || 4ll * (n - 1) < tiles));
-                        if (n > 1) CHECK((unsigned long long)r * kv * g * n <= paged_workspace_records(rows, kv * g, kv));
+                    for (long long keys : {1ll, 17ll, 512ll, 1024ll, 1025ll, 5000ll, 2147483647ll}) {
+                        const unsigned long long most = paged_workspace_records(rows, kv * g, kv);
+                        for (int kt : {16, 32}) for (long long room : {keys, 2147483647ll}) {
+                            const DecodePlan p = paged_decode_plan(r, kv * g, kv, kt, keys, room);
+                            if (p.shares) CHECK(r * (room / kt + 3) <= 2147483647ll);
+                            CHECK(p.blocks == (g + 15) / 16 && p.shares >= 0 && p.records <= most);
+                            // a record for every wave, of its first and its last sequence, and query head
+                            if (p.shares) CHECK(p.records == 2ull * p.shares * kv * p.blocks * (g < 16 ? g : 16) && r <= kPagedShareRows && r * kv * p.blocks <= kPagedCounters);
+                        }
+                        // prefill: r rows of one entry
+                        const long long units = (r * g / 128 + 1) * kv;
+                        const int n = paged_prefill_splits(units, (keys + 31) / 32);
+                        CHECK(n >= 1 && n <= kPagedMaxSplits);
+                        if (n > 1) CHECK((unsigned long long)r * kv * g * n <= most);
                     }
     return 0;
 }

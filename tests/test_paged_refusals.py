@@ -87,6 +87,8 @@ def test_attention_workspace_and_the_rest():
     assert decode(c=big, ws=A + 4, size=need) == EINVAL
     assert _lib.load().uocr_hip_paged_attention_workspace_size(C.byref(big), 3, 3) == 0
     assert _lib.load().uocr_hip_paged_attention_workspace_size(C.byref(big), 4, -1) == 0
+    init = _lib.load().uocr_hip_paged_attention_workspace_init
+    assert init(None, need, None) == EINVAL and init(A + 8, need, None) == EINVAL and init(A, 1024, None) == EWORKSPACE
     assert prefill(start=None) == EINVAL and prefill(n=-1) == EINVAL
     assert prefill(o=opts(window=4, causal=0)) == EINVAL
     assert prefill(n=2**30, o=opts(heads=4)) == EUNSUPPORTED
@@ -159,6 +161,16 @@ def test_frequencies():
     # the ramp's ends are whole indices: one index of leeway beyond the turn limits
     assert np.array_equal(h[kept], f[kept].astype(np.float32)) and np.array_equal(h[div][1:], (f[div] / 8).astype(np.float32)[1:])
     assert (np.diff(h / f.astype(np.float32)) <= 1e-6).all()
+
+
+def test_packed_structs():
+    a = RowsC(A + 16, 2, 2**40, 3)
+    b = AttentionOptsC(32, 0.5, 30.0, A, 1, 77, 2 * A, 1, 3 * A, 4 * A)
+    assert _lib.ROWS_PACK(A + 16, 2, 2**40, 3) == bytes(a)
+    packed = _lib.OPTS_PACK(32, 0.5, 30.0, A, True, 77, 2 * A, True, 3 * A, 4 * A)
+    again = AttentionOptsC.from_buffer_copy(packed)
+    assert len(packed) == C.sizeof(AttentionOptsC)
+    assert all(getattr(again, n) == getattr(b, n) for n, _ in AttentionOptsC._fields_)
 
 
 def test_python_refuses_before_the_library():

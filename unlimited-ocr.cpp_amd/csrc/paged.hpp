@@ -13,7 +13,12 @@ namespace uocr_hip {
 #define UOCR_HD
 #endif
 
-constexpr int kPagedTarget = 2048;    // workgroups that a split call aims at
+constexpr int kPagedShareRows = 1024;   // sequences of a decode call that is cut into shares
+constexpr int kPagedShareGroups = 256;  // workgroups that it aims at: one per CU
+constexpr int kPagedCounters = 16384;   // (sequence, KV head, 16 query heads) of such a call
+constexpr int kPagedMagic = 0x70616765; // first word of a workspace that was set up
+constexpr int kPagedHead = 64 + kPagedCounters * 4;  // bytes before a workspace's partial results
+constexpr int kPagedUnitTiles = 8;     // tiles of keys that one workgroup takes alone
 constexpr int kPagedPrefillTarget = 512;
 constexpr int kPagedMaxSplits = 128;
 
@@ -109,14 +114,28 @@ UOCR_HD inline TileWalk tile_walk(const Span& s) {
     return w;
 }
 
-// Splits of a decode call of `units` (sequence, KV head, 16 query heads) with
-// `tiles` tiles of keys at most: enough workgroups for the chip, each of its
-// 4 waves with a tile at least.
-inline int paged_splits(long long units, long long tiles) {
-    const long long want = (kPagedTarget + units - 1) / units, most = (tiles + 3) / 4;
-    long long n = want < most ? want : most;
-    if (n > kPagedMaxSplits) n = kPagedMaxSplits;
-    return n < 1 ? 1 : (int)n;
+// How a decode call is shared out: one workgroup per (sequence, KV head, 16 query heads) where
+// `max_keys` is short or the rows (or the `room` for their keys) too many for the shares' table, else (shares > 0) equal
+// shares of all rows' tiles, one workgroup per share and KV head, and a join.
+// A workgroup of 8 waves takes 8 tiles at a time.
+struct DecodePlan {
+    int blocks;   // of 16 query heads per KV head
+    int shares;   // 0: one workgroup per unit
+    unsigned long long records;  // partial results of one (workgroup, first or last sequence, query head) each
+};
+inline DecodePlan paged_decode_plan(long long batch, int heads, int kv_heads, int tile_keys, long long max_keys, long long room) {
+    DecodePlan p{(heads / kv_heads + 15) / 16, 0, 0};
+    if (batch > kPagedShareRows || max_keys <= kPagedUnitTiles * tile_keys) return p;
+    const long long kvb = (long long)kv_heads * p.blocks;
+    // (a row has two more tiles than its keys fill at most, and the line's length is an int)
+    if (batch * kvb > kPagedCounters || batch * (room / tile_keys + 3) > 0x7fffffff) return p;
+    const long long tiles = batch * ((max_keys + tile_keys - 1) / tile_keys);
+    long long n = kPagedShareGroups / kvb;  // (no more than the chip holds at once)
+    if (n < 1) n = 1;
+    if (n > tiles) n = tiles;
+    p.shares = (int)n;
+    p.records = (unsigned long long)n * kvb * 2 * (heads / kv_heads < 16 ? heads / kv_heads : 16);
+    return p;
 }
 
 // Splits of a prefill call of `units` (tile, KV head) workgroups: where they leave most of
@@ -128,17 +147,14 @@ inline int paged_prefill_splits(long long units, long long tiles) {
     return n < 1 ? 1 : (int)n;
 }
 
-// Partial results (row, head, split) that a call of up to `rows` rows may hold.
-// Decode: one row per unit of up to 16 heads; units * splits stays below kPagedTarget + units, and
-// calls of kPagedTarget units are not split. Prefill: a unit is 128 (row, head) pairs of a KV head at most, and
-// units * splits stays below kPagedPrefillTarget.
+// Partial results that calls of up to `rows` rows may hold. Decode: 2 per workgroup and query head;
+// prefill: a unit is 128 (row, head) pairs of a KV head at most, and units * splits stays below
+// kPagedPrefillTarget.
 inline unsigned long long paged_workspace_records(long long rows, int heads, int kv_heads) {
-    const long long group = heads / kv_heads, blocks = (group + 15) / 16;
-    const long long full = kPagedTarget / (kv_heads * blocks) + 1;  // rows of a call that is not split
-    const long long any = rows * heads * kPagedMaxSplits;
-    long long decode = heads * (full + (rows < full ? rows : full)), prefill = 128ll * kPagedPrefillTarget;
-    const long long most = decode > prefill ? decode : prefill;
-    return (unsigned long long)(any < most ? any : most);
+    const long long group = heads / kv_heads, kvb = kv_heads * ((group + 15) / 16), cols = group < 16 ? group : 16;
+    const long long decode = (kPagedShareGroups + kvb) * 2 * cols;
+    const long long all = rows * heads * kPagedMaxSplits, most = 128ll * kPagedPrefillTarget, prefill = all < most ? all : most;
+    return (unsigned long long)(decode > prefill ? decode : prefill);
 }
 
 }  // namespace uocr_hip

@@ -47,19 +47,26 @@ int paged_rows(const char* what, const uocr_hip_rows* r, bool vec, PagedRows* ou
     return UOCR_HIP_OK;
 }
 
-int paged_take_workspace(PagedAttnArgs& a, int rows, void* ws, size_t ws_bytes) {
-    if (a.n_splits <= 1) return UOCR_HIP_OK;
-    const size_t records = (size_t)rows * a.heads * a.n_splits, need = records * (a.head_dim + 2) * sizeof(float);
+int paged_take_workspace(PagedAttnArgs& a, size_t records, int rows, void* ws, size_t ws_bytes) {
+    const size_t need = kPagedHead + records * (a.head_dim + 2) * sizeof(float) + rows * 2 * sizeof(int);
     if (!ws || ws_bytes < need)
         return set_error(UOCR_HIP_EWORKSPACE, "attention: workspace of " + std::to_string(ws ? ws_bytes : 0) + " bytes, " +
                                                   std::to_string(need) + " needed");
     if ((uintptr_t)ws % 16) return set_error(UOCR_HIP_EINVAL, "attention: workspace must be 16-byte aligned");
-    a.part = static_cast<float*>(ws);
+    // one word before the counters, on their cache line
+    a.counters = static_cast<int*>(ws) + 1;
+    a.part = reinterpret_cast<float*>(static_cast<char*>(ws) + kPagedHead);
     a.part_ml = a.part + records * a.head_dim;
+    a.part_rows = reinterpret_cast<int*>(a.part_ml + 2 * records);
     return UOCR_HIP_OK;
 }
 
 namespace {
+
+__global__ __launch_bounds__(256) void paged_workspace_kernel(int* ws) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < kPagedHead / 4) ws[i] = i ? 0 : kPagedMagic;
+}
 
 int attn_args(const uocr_hip_paged_cache* cache, const uocr_hip_attention_opts* o, const uocr_hip_rows* q,
               const uocr_hip_rows* out, int rows, int batch, const int* d_seqs, const int* d_kv_len, int max_kv_len,
@@ -122,7 +129,19 @@ size_t uocr_hip_paged_attention_workspace_size(const uocr_hip_paged_cache* cache
         set_error(UOCR_HIP_EINVAL, "workspace: heads must be a positive multiple of kv_heads, rows >= 0");
         return 0;
     }
-    return paged_workspace_records(rows, heads, cache->kv_heads) * (cache->head_dim + 2) * sizeof(float);
+    return kPagedHead + paged_workspace_records(rows, heads, cache->kv_heads) * (cache->head_dim + 2) * sizeof(float) +
+           std::min(rows, kPagedShareRows) * 2 * sizeof(int);
+}
+
+int uocr_hip_paged_attention_workspace_init(void* workspace, size_t workspace_bytes, void* stream) {
+    if (!workspace || (uintptr_t)workspace % 16)
+        return set_error(UOCR_HIP_EINVAL, "workspace: null or not 16-byte aligned");
+    if (workspace_bytes < kPagedHead) return set_error(UOCR_HIP_EWORKSPACE, "workspace: too small");
+    launch_k(paged_workspace_kernel, dim3(kPagedHead / 4 / 256 + 1), dim3(256), 0, (hipStream_t)stream,
+             static_cast<int*>(workspace));
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? UOCR_HIP_OK
+                           : set_error(UOCR_HIP_EHIP, std::string("workspace launch: ") + hipGetErrorString(e));
 }
 
 int uocr_hip_paged_attention_decode(const uocr_hip_paged_cache* cache, const uocr_hip_attention_opts* opts,

@@ -35,10 +35,12 @@ struct PagedAttnArgs {
     const int* kv_len;   // [n_seqs]
     PagedScores sc;
     MaskArgs mask;
-    int chunk;     // tiles of keys per split
-    int n_splits;  // splits that the grid has room for
-    float* part;   // [rows][heads][n_splits][head_dim] sums of p v, then [rows][heads][n_splits][2] (max, sum)
-    float* part_ml;
+    int n_splits;  // prefill: splits of the keys; decode: shares (0: one workgroup per unit)
+    float* part;   // partial results: sums of p v [records][head_dim], then
+    float* part_ml;  // [records][2]: maximum and sum, then
+    int* counters;   // (decode) [batch][KV heads x blocks of 16 heads]: sums that are there (0 between calls);
+                     // the workspace's first word before them. Null: joined by a kernel of its own
+    int* part_rows;  // (decode) [batch][2]: first and last share with tiles of a row
     int n_tiles;   // (prefill) query tiles that the grid has room for
 };
 

@@ -24,7 +24,7 @@ int paged_rows(const char* what, const uocr_hip_rows* r, bool vec, PagedRows* ou
 int launch_paged_decode(PagedAttnArgs a, int dtype, long long max_keys, void* ws, size_t ws_bytes, hipStream_t st);
 int launch_paged_prefill(PagedAttnArgs a, int dtype, long long max_keys, void* ws, size_t ws_bytes, hipStream_t st);
 
-// Gives a call with a.n_splits > 1 its place for rows * heads * n_splits partial results
-int paged_take_workspace(PagedAttnArgs& a, int rows, void* ws, size_t ws_bytes);
+// Gives a call its place for `records` partial results and (decode) `rows` entries about rows
+int paged_take_workspace(PagedAttnArgs& a, size_t records, int rows, void* ws, size_t ws_bytes);
 
 }  // namespace uocr_hip

@@ -1,6 +1,7 @@
 """ctypes loader and signatures for libuocr_hip.so."""
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # UOCR_HIP_LIB overrides the in-tree library (used to compare builds)
@@ -76,6 +77,11 @@ class AttentionOptsC(C.Structure):
                 ("key_begin", C.c_void_p), ("key_end", C.c_void_p)]
 
 
+# RowsC and AttentionOptsC as bytes, for calls that pass them by address (a third of a Structure's time)
+ROWS_PACK = struct.Struct("@Piqq").pack
+OPTS_PACK = struct.Struct("@iffPiiPiPP").pack
+
+
 def lib_path():
     return _LIB_PATH
 
@@ -143,6 +149,7 @@ SIGNATURES = {
     "uocr_hip_rope": (C.c_int, [C.c_void_p] * 2 + [C.c_int] * 4 + [C.c_void_p] * 2 + [C.c_int] * 2 + [C.c_float] + [C.c_void_p] * 3),
     "uocr_hip_rope_append_paged": (C.c_int, [C.c_void_p] * 3 + [C.c_int] * 2 + [C.c_void_p] * 2 + [C.c_int] * 2 + [C.c_float] + [C.c_void_p] * 5),
     "uocr_hip_paged_attention_workspace_size": (C.c_size_t, [C.c_void_p, C.c_int, C.c_int]),
+    "uocr_hip_paged_attention_workspace_init": (C.c_int, [C.c_void_p, C.c_size_t, C.c_void_p]),
     "uocr_hip_paged_attention_decode": (C.c_int, [C.c_void_p] * 3 + [C.c_int] + [C.c_void_p] * 2 + [C.c_int] + [C.c_void_p] * 2 + [C.c_size_t, C.c_void_p]),
     "uocr_hip_paged_attention_prefill": (C.c_int, [C.c_void_p] * 3 + [C.c_int] * 2 + [C.c_void_p] * 3 + [C.c_int] + [C.c_void_p] * 2 + [C.c_size_t, C.c_void_p]),
     "uocr_hip_moe_router_topk": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int,
