@@ -161,7 +161,7 @@ def run_decode(dev, rng, pool, heads, out_dtype=None, seqs=None, spread=1.5, str
                     begin=host["key_begin"][i] if "key_begin" in host else 0,
                     end=host["key_end"][i] if "key_end" in host else None)
         want, bound = R.attend(q[i], pool.k[b], pool.v[b], pool.lens[b] - 1, out_dtype, pool.dtype, P_ERR[pool.dtype],
-                               scale=kw.get("scale"), softcap=kw.get("softcap", 0.0),
+                               scale=kw.get("scale"), softcap=kw.get("softcap", 0.0), fast_cap=pool.dtype != "f32",
                                slopes=arg["slopes"].cpu().numpy() if arg.get("slopes") is not None else None, **mask)
         R.close(out[i], want, bound)
     return out

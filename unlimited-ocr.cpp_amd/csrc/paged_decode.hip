@@ -225,7 +225,7 @@ struct DecodeWave {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int key = h * 16 + g * 4 + i;
-                    float x = score2<CAP, BIAS, true>(s[h][i], a.sc, slope2, dist0 - key);
+                    float x = score2<CAP, BIAS, F32>(s[h][i], a.sc, slope2, dist0 - key);
                     if (lost >> key & 1) x = NAN;
                     p[h][i] = seen >> key & 1 ? x : -INFINITY;
                     top = fmaxf(top, p[h][i]);
