@@ -104,10 +104,12 @@ static int splits() {
                             if (p.shares) CHECK(p.records == 2ull * p.shares * kv * p.blocks * (g < 16 ? g : 16) && r <= kPagedShareRows && r * kv * p.blocks <= kPagedCounters);
                         }
                         // prefill: r rows of one entry
-                        const long long units = (r * g / 128 + 1) * kv;
-                        const int n = paged_prefill_splits(units, (keys + 31) / 32);
-                        CHECK(n >= 1 && n <= kPagedMaxSplits);
-                        if (n > 1) CHECK((unsigned long long)r * kv * g * n <= most);
+                        for (int d : {8, 128, 256}) for (int f32 : {0, 1}) {
+                            const PrefillPlan p = paged_prefill_plan(r, 1, kv * g, kv, d, f32, keys);
+                            CHECK(p.row_waves == 4 || p.row_waves == 2 || p.row_waves == 1);
+                            CHECK(p.tiles * p.row_waves * 32 >= r * g && p.splits >= 1 && p.splits <= kPagedMaxSplits);
+                            if (p.splits > 1) CHECK((unsigned long long)r * kv * g * p.splits <= most);
+                        }
                     }
     return 0;
 }

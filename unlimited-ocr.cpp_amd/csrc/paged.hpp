@@ -19,7 +19,7 @@ constexpr int kPagedCounters = 16384;   // (sequence, KV head, 16 query heads) o
 constexpr int kPagedMagic = 0x70616765; // first word of a workspace that was set up
 constexpr int kPagedHead = 64 + kPagedCounters * 4;  // bytes before a workspace's partial results
 constexpr int kPagedUnitTiles = 8;     // tiles of keys that one workgroup takes alone
-constexpr int kPagedPrefillTarget = 512;
+constexpr int kPagedPrefillTarget = 512;  // workgroups that a split prefill call aims at
 constexpr int kPagedMaxSplits = 128;
 
 // n / d for 0 <= n < 2^31 by a multiplication: with s = ceil(log2 d) and
@@ -138,13 +138,38 @@ inline DecodePlan paged_decode_plan(long long batch, int heads, int kv_heads, in
     return p;
 }
 
-// Splits of a prefill call of `units` (tile, KV head) workgroups: where they leave most of
-// the chip idle, each split with 4 tiles of keys at least.
-inline int paged_prefill_splits(long long units, long long tiles) {
-    const long long want = kPagedPrefillTarget / units, most = tiles / 4;
+// How a prefill call is shared out: workgroups of 4 waves, `row_waves` of them along the (row, head)
+// pairs of a KV head (32 each), the others on other tiles of keys; `tiles` of pairs per KV head at
+// most (each entry rounds up by less than one); the keys split over `splits` workgroups where
+// those leave most of the chip idle, 256 keys in each at least.
+// 128 pairs per workgroup share K and V best, 64 or 32 leave fewer rounds one after the other and more
+// workgroups: they are for calls that do not fill the chip, and need keys for every wave. us with 4 / 2 / 1 row
+// waves, head_dim 128 (workgroups of 128 pairs):
+//   bf16  10 heads, 64 rows (10) 8.2 / 9.9 / 12.1, 256 (30) 14.2 / 12.8 / 12.7, 1024 (90) 36 / 31 / 29,
+//         4096 (330) 133 / 102 / 198; 32 heads over 8, 1024 rows (264) 39 / 32 / 70, 4096 (1032) 191 / 239 / 583
+//   f32   10 heads, 64 rows 17.0 / 14.7 / 16.3, 256 47 / 34 / 24, 1024 93 / 77 / 65, 4096 718 / 594 / 589;
+//         32 heads over 8, 1024 rows 166 / 135 / 153, 4096 1238 / 1322 / 1770
+// Heads above 128 have no room for it (registers, LDS).
+struct PrefillPlan {
+    int row_waves, splits;
+    long long tiles;
+};
+inline PrefillPlan paged_prefill_plan(long long rows, long long batch, int heads, int kv_heads, int head_dim, bool f32,
+                                      long long max_keys) {
+    const long long pairs = rows * (heads / kv_heads);
+    const auto tiles = [&](int rw) { return pairs / (32 * rw) + batch; };
+    const auto groups = [&](int rw) { return tiles(rw) * kv_heads; };
+    PrefillPlan p{4, 1, 0};
+    if (head_dim <= 128) {
+        if (f32 && groups(1) < 512 && max_keys > 96) p.row_waves = 1;
+        else if (groups(4) < (f32 ? 1024 : 512) && max_keys > (f32 ? 32 : 64)) p.row_waves = 2;
+    }
+    p.tiles = tiles(p.row_waves);
+    const long long units = groups(p.row_waves), want = kPagedPrefillTarget / units, most = max_keys / 256;
     long long n = want < most ? want : most;
     if (n > kPagedMaxSplits) n = kPagedMaxSplits;
-    return n < 1 ? 1 : (int)n;
+    p.splits = n < 1 ? 1 : (int)n;
+    return p;
 }
 
 // Partial results that calls of up to `rows` rows may hold. Decode: 2 per workgroup and query head;

@@ -5,7 +5,8 @@
 // keys with a running maximum and sum per row. Bound by the matrix cores: 4 head_dim
 // operations per visible pair and head.
 //
-// A workgroup of 4 waves takes 128 query rows of one KV head: the `group` query heads that
+// A workgroup of 4 waves takes 128 query rows of one KV head (64 or 32 in small calls, the waves
+// then also taking turns at the tiles of keys): the `group` query heads that
 // share it side by side for each token, so that K and V tiles serve all of them. Tiles of
 // 64 keys (32 for f32) go through registers into LDS, the next one in flight during the
 // current one's products; registers (and not a direct load) because pages may
@@ -28,35 +29,39 @@
 #include "launch.hpp"
 #include "paged_device.hpp"
 #include "paged_host.hpp"
-#include "xcd_order.hpp"
 
 namespace uocr_hip {
 
-constexpr int kPreRows = 128;  // packed query rows per workgroup
 constexpr int kPreWaves = 4;
-template <typename T>
-constexpr int kPreKeys = sizeof(T) == 4 ? 32 : 64;  // keys per tile
 
-template <typename T, int DP>
+// RW: waves along the rows; the other 4 / RW groups of waves take other tiles of keys
+template <typename T, int DP, int RW>
 struct PreShape {
-    static constexpr int ES = sizeof(T);
+    static constexpr int ES = sizeof(T), KW = kPreWaves / RW;
+    static constexpr int ROWS = RW * 32;  // packed query rows per workgroup
+    static constexpr int KEYS = ES == 4 ? 32 : 64;  // per tile
     static constexpr int KSTR = DP * ES + 16;
     static constexpr int VPAD = ES == 4 ? 32 : (DP * 2 % 256 == 64 || DP * 2 % 256 == 192) ? 0 : 64;
     static constexpr int VSTR = DP * ES + VPAD;
-    static constexpr int BYTES = kPreKeys<T> * (KSTR + VSTR);  // one buffer
+    static constexpr int TILE = KEYS * (KSTR + VSTR);
+    static constexpr int BUFS = KW == 1 ? 2 : 1;
+    static constexpr int LDS = TILE * KW * BUFS;
+    // workgroups per CU that registers and LDS allow
+    static constexpr int RESIDENT = DP > 128 || KW == 4 ? 1 : 2;
 };
 
 // Row range of sequence entry b in [0, rows]
 __device__ __forceinline__ int pre_start(const PagedAttnArgs& a, int b) { return imin(imax(a.q_start[b], 0), a.rows); }
 
 // Entry b and tile within it of tile index t (tiles of entry after entry); -1: none
+template <int ROWS>
 __device__ __forceinline__ int pre_find(const PagedAttnArgs& a, int t, int& tile) {
     const int lane = threadIdx.x & 63;
     int before = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
         const int b = b0 + lane;
         int n = 0;
-        if (b < a.batch) n = (imax(pre_start(a, b + 1) - pre_start(a, b), 0) * a.group + kPreRows - 1) / kPreRows;
+        if (b < a.batch) n = (imax(pre_start(a, b + 1) - pre_start(a, b), 0) * a.group + ROWS - 1) / ROWS;
         int sum = n;
 #pragma unroll
         for (int x = 1; x < 64; x *= 2) {
@@ -101,29 +106,29 @@ __device__ __forceinline__ s16x4 lds_tr(const char* p) {
         (__attribute__((address_space(3))) s16x4*)(__attribute__((address_space(3))) void*)(void*)p);
 }
 
-template <typename T, int DP, bool CAP, bool BIAS>
-__global__ __launch_bounds__(kPreWaves * 64, DP > 128 ? 1 : 2) void paged_prefill_kernel(PagedAttnArgs a) {
+template <typename T, int DP, bool CAP, bool BIAS, int RW>
+__global__ __launch_bounds__(kPreWaves * 64, (PreShape<T, DP, RW>::RESIDENT)) void paged_prefill_kernel(PagedAttnArgs a) {
+    typedef PreShape<T, DP, RW> P;
     constexpr bool F32 = sizeof(T) == 4;
-    constexpr int ES = sizeof(T), BN = kPreKeys<T>, KB = BN / 32, CH = DP * ES / 16, NL = BN * CH / (kPreWaves * 64);
-    static_assert(BN * CH % (kPreWaves * 64) == 0, "whole 16-byte units per thread");
-    constexpr int KSTR = PreShape<T, DP>::KSTR, VSTR = PreShape<T, DP>::VSTR, BUF = PreShape<T, DP>::BYTES;
+    constexpr int ES = sizeof(T), BN = P::KEYS, KB = BN / 32, CH = DP * ES / 16, KW = P::KW, GT = RW * 64, NL = BN * CH / GT;
+    static_assert(BN * CH % GT == 0, "whole 16-byte units per thread");
+    constexpr int KSTR = P::KSTR, VSTR = P::VSTR;
     constexpr int NF = F32 ? DP / 8 : DP / 16;  // 16-byte pieces of a query row per lane
     constexpr int DB = DP / 32;
     typedef typename Vec8<T>::type vec_t;
-    extern __shared__ __attribute__((aligned(16))) char s_buf[];  // two buffers: K rows, then V rows
+    extern __shared__ __attribute__((aligned(16))) char s_buf[];  // tiles: K rows, then V rows
     __shared__ int s_range[kPreWaves][4];
     __shared__ int s_lost;
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 31, h = lane >> 5;
-    // Items (KV head, tile), an eighth in order per XCD: a KV head's tiles share
-    // its K and V in one L2. Last tiles first: they see the most keys under a causal mask.
-    const int items = a.n_tiles * a.kv_heads, per = gridDim.x / a.n_splits;
-    const int split = blockIdx.x / per, blk = blockIdx.x % per, xcd = blk % kXcds;
-    const int first = xcd_first_item(xcd, items), item = first + blk / kXcds;
-    if (item >= xcd_first_item(xcd + 1, items)) return;
-    const int kvh = item / a.n_tiles;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 31, h = lane >> 5;
+    const int rw = wave % RW, kg = wave / RW, gtid = tid % GT;
+    // Last tiles first: they see the most keys under a causal mask. The KV heads of a tile side by
+    // side: workgroup b runs on XCD b % 8, so 8 of them leave each XCD's L2 one head's K and V, and other
+    // numbers of heads share every XCD's evenly (runs of one head per XCD: 4096 rows of 10 heads 158 us, this way 113).
+    const int per = a.n_tiles * a.kv_heads, split = blockIdx.x / per, item = blockIdx.x % per;
+    const int kvh = item % a.kv_heads;
     int tile;
-    const int entry = pre_find(a, a.n_tiles - 1 - item % a.n_tiles, tile);
+    const int entry = pre_find<P::ROWS>(a, a.n_tiles - 1 - item / a.kv_heads, tile);
     if (entry < 0) return;
     const int seq = a.seqs ? a.seqs[entry] : entry;
     if ((uint32_t)seq >= (uint32_t)a.c.n_seqs) return;
@@ -133,7 +138,7 @@ __global__ __launch_bounds__(kPreWaves * 64, DP > 128 ? 1 : 2) void paged_prefil
     const int len = gone ? 0 : imax(kv, 0);
 
     // this lane's query row
-    const int packed = tile * kPreRows + wave * 32 + i;
+    const int packed = tile * P::ROWS + rw * 32 + i;
     const bool live = packed < n * a.group;
     const int token = packed / a.group, row = start + imin(token, n - 1), head = kvh * a.group + packed % a.group;
     const int pos = len - n + token;
@@ -218,7 +223,7 @@ __global__ __launch_bounds__(kPreWaves * 64, DP > 128 ? 1 : 2) void paged_prefil
     auto load = [&](long long off) {
 #pragma unroll
         for (int e = 0; e < NL; ++e) {
-            const int u = e * (kPreWaves * 64) + tid, r = u / CH, c = u % CH;
+            const int u = e * GT + gtid, r = u / CH, c = u % CH;
             const long long at = shfl64(off, r) + c * 16;
             kw[e] = vw[e] = u32x4{0, 0, 0, 0};
             if (c * (16 / ES) < a.head_dim) {
@@ -230,7 +235,7 @@ __global__ __launch_bounds__(kPreWaves * 64, DP > 128 ? 1 : 2) void paged_prefil
     auto store = [&](char* buf) {
 #pragma unroll
         for (int e = 0; e < NL; ++e) {
-            const int u = e * (kPreWaves * 64) + tid, r = u / CH, c = u % CH;
+            const int u = e * GT + gtid, r = u / CH, c = u % CH;
             *reinterpret_cast<u32x4*>(buf + r * KSTR + c * 16) = kw[e];
             *reinterpret_cast<u32x4*>(buf + BN * KSTR + r * VSTR + c * 16) = vw[e];
         }
@@ -238,27 +243,33 @@ __global__ __launch_bounds__(kPreWaves * 64, DP > 128 ? 1 : 2) void paged_prefil
 
     float m = -INFINITY, l = 0.0f;  // of row i (l: over this lane's keys), in log 2
     f32x16 o[DB] = {};
-    if (t_begin < t_end) {
-        load(place(t_begin));
-        long long next = t_begin + 1 < t_end ? place(t_begin + 1) : 0;
-        store(s_buf);
-        for (int t = t_begin; t < t_end; ++t) {
-            __syncthreads();
-            const char* buf = s_buf + ((t - t_begin) & 1) * BUF;
-            if (t + 1 < t_end) load(next);
-            if (t + 2 < t_end) next = place(t + 2);
-            const int base = tile_base(t);
+    const int rounds = (t_end - t_begin + KW - 1) / KW;  // (the same for every wave: barriers)
+    if (rounds) {
+        // group kg: tiles t_begin + kg, + KW, ..
+        int t = t_begin + kg;
+        char* const own = s_buf + kg * P::TILE;
+        if (t < t_end) load(place(t));
+        long long next = t + KW < t_end ? place(t + KW) : 0;
+        if (t < t_end) store(own);
+        for (int round = 0; round < rounds; ++round, t += KW) {
+            // one wave per group: its tile is its own, and LDS accesses of a wave stay in order
+            if constexpr (RW > 1) __syncthreads();
+            const char* buf = own + (P::BUFS == 2 ? (round & 1) * P::TILE : 0);
+            if (t + KW < t_end) load(next);
+            if (t + 2 * KW < t_end) next = place(t + 2 * KW);
+            if (t < t_end) {
+                const int base = tile_base(t);
             const uint64_t seen = bits(span.b0 - base, span.e0 - base) | bits(span.b1 - base, span.e1 - base);
             constexpr uint64_t kAll = BN == 64 ? ~0ull : (1ull << BN) - 1;
             if (__any((seen & kAll) != 0)) {
                 f32x16 s[KB];
 #pragma unroll
-                for (int b = 0; b < KB; ++b) {
-                    s[b] = f32x16{};
-                    const char* kp = buf + (b * 32 + i) * KSTR + h * 16;
+                for (int b = 0; b < KB; ++b) s[b] = f32x16{};
 #pragma unroll
-                    for (int f = 0; f < NF; ++f) {
-                        const vec_t k = *reinterpret_cast<const vec_t*>(kp + f * 32);
+                for (int f = 0; f < NF; ++f)
+#pragma unroll
+                    for (int b = 0; b < KB; ++b) {
+                        const vec_t k = *reinterpret_cast<const vec_t*>(buf + (b * 32 + i) * KSTR + h * 16 + f * 32);
                         if constexpr (F32) {
 #pragma unroll
                             for (int e = 0; e < 4; ++e) s[b] = mfma_32x32x2(k[e], q[f][e], s[b]);
@@ -266,7 +277,6 @@ __global__ __launch_bounds__(kPreWaves * 64, DP > 128 ? 1 : 2) void paged_prefil
                             s[b] = mfma_32x32x16(k, q[f], s[b]);
                         }
                     }
-                }
                 const bool whole = __all((seen & kAll) == kAll);
                 if constexpr (CAP || BIAS) {
                     const int dist0 = pos - base - 4 * h;
@@ -339,10 +349,43 @@ __global__ __launch_bounds__(kPreWaves * 64, DP > 128 ? 1 : 2) void paged_prefil
                     }
                 }
             }
-            if (t + 1 < t_end) store(s_buf + ((t + 1 - t_begin) & 1) * BUF);
+            }
+            if constexpr (RW > 1 && P::BUFS == 1) __syncthreads();
+            if (t + KW < t_end) store(own + (P::BUFS == 2 ? (round + 1 & 1) * P::TILE : 0));
         }
     }
     __syncthreads();
+    // the groups' sums of the same rows, by halves
+#pragma unroll
+    for (int half = KW / 2; half >= 1; half /= 2) {
+        f32x4* at = reinterpret_cast<f32x4*>(s_buf) + (size_t)(kg % half * RW + rw) * (DB * 4 + 1) * 64 + lane;
+        static_assert(KW == 1 || (DB * 4 + 1) * 1024 * (kPreWaves / 2) <= P::LDS, "half the waves' sums fit");
+        if (kg >= half && kg < 2 * half) {
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) at[(d * 4 + r / 4) * 64] = f32x4{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
+            at[DB * 4 * 64] = f32x4{m, l, 0.0f, 0.0f};
+        }
+        __syncthreads();
+        if (kg < half) {
+            const f32x4 ml = at[DB * 4 * 64];
+            const float up = fmaxf(m, ml[0]), ref = up == -INFINITY ? 0.0f : up;
+            const float f1 = __builtin_amdgcn_exp2f(m - ref), f2 = __builtin_amdgcn_exp2f(ml[0] - ref);
+            m = up;
+            l = l * f1 + ml[1] * f2;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    const f32x4 v = at[(d * 4 + r / 4) * 64];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[d][r + e] = o[d][r + e] * f1 + v[e] * f2;
+                }
+        }
+        __syncthreads();
+    }
+    if (kg) return;
     l += __shfl_xor(l, 32, 64);
     if (a.n_splits > 1) {
         if (live) {
@@ -386,39 +429,38 @@ __global__ __launch_bounds__(kPreWaves * 64, DP > 128 ? 1 : 2) void paged_prefil
     const uint64_t keep = __ballot(live) & ~again;
     // rows through LDS, so that a row leaves in 16-byte pieces side by side (8-byte pieces of
     // 32 rows per store: 6 us for 64 rows of 32 heads instead of 1)
-    const int oes = F32 || a.out_f32 ? 4 : ES, ostr = DP * oes + 16;
-    static_assert(kPreWaves * 32 * (DP * 4 + 16) <= 2 * BUF, "a workgroup's rows fit its buffers");
-    char* so = s_buf + wave * 32 * ostr;
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            const int d0 = d * 32 + 2 * r + 4 * h;
-            const f32x4 v = {o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
-            if (F32 || a.out_f32) {
-                *reinterpret_cast<f32x4*>(so + i * ostr + d0 * 4) = v;
-            } else {
-                T t[4] = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
-                __builtin_memcpy(__builtin_assume_aligned(so + i * ostr + d0 * ES, 8), t, 8);
-            }
-        }
-    const int per_row = a.head_dim * oes / 16;  // 16-byte pieces of a row
+    static_assert(P::ROWS * (DP * 4 + 16) <= P::LDS, "a workgroup's rows fit its tiles");
     const bool wide = (((uintptr_t)a.out.p | a.out.row_bytes | a.out.head_bytes) & 15) == 0;
     const long long out_at = row * a.out.row_bytes + head * a.out.head_bytes;
-    for (int u = lane; u < (32 * per_row + 63) / 64 * 64; u += 64) {
-        const int r = imin(u / per_row, 31), c = u % per_row;
-        char* p = a.out.p + shfl64(out_at, r) + c * 16;
-        if (u >= 32 * per_row || !(keep >> r & 1)) continue;
-        const u32x4 v = *reinterpret_cast<const u32x4*>(so + r * ostr + c * 16);
-        if (wide) {
-            *reinterpret_cast<u32x4*>(p) = v;
-        } else {
-            for (int e = 0; e < 16 / oes; ++e) {
-                if (oes == 4) reinterpret_cast<uint32_t*>(p)[e] = v[e];
-                else reinterpret_cast<uint16_t*>(p)[e] = (uint16_t)(v[e / 2] >> (16 * (e & 1)));
+    const auto put = [&](auto type) {
+        typedef decltype(type) O;
+        constexpr int OES = sizeof(O), OSTR = DP * OES + 16, PIECES = DP * OES / 16;
+        char* so = s_buf + rw * 32 * OSTR;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                O t[4] = {(O)o[d][r], (O)o[d][r + 1], (O)o[d][r + 2], (O)o[d][r + 3]};
+                __builtin_memcpy(__builtin_assume_aligned(so + i * OSTR + (d * 32 + 2 * r + 4 * h) * OES, 4 * OES), t, 4 * OES);
+            }
+#pragma unroll 4
+        for (int u = lane; u < 32 * PIECES; u += 64) {
+            const int r = u / PIECES, c = u % PIECES;
+            char* p = a.out.p + shfl64(out_at, r) + c * 16;
+            if (c * (16 / OES) >= a.head_dim || !(keep >> r & 1)) continue;
+            const u32x4 v = *reinterpret_cast<const u32x4*>(so + r * OSTR + c * 16);
+            if (wide) {
+                *reinterpret_cast<u32x4*>(p) = v;
+            } else {
+                for (int e = 0; e < 16 / OES; ++e) {
+                    if constexpr (OES == 4) reinterpret_cast<uint32_t*>(p)[e] = v[e];
+                    else reinterpret_cast<uint16_t*>(p)[e] = (uint16_t)(v[e / 2] >> (16 * (e & 1)));
+                }
             }
         }
-    }
+    };
+    if (F32 || a.out_f32) put(0.0f);
+    else put((T)0.0f);
     for (; again; again &= again - 1) {
         const int src = __builtin_ctzll(again);
         row_attention<T>(a, seq, __shfl(row, src, 64), __shfl(head, src, 64), __shfl(pos, src, 64), len, gone);
@@ -475,10 +517,10 @@ __global__ __launch_bounds__(256) void paged_prefill_join_kernel(PagedAttnArgs a
         if (lane + 64 * e < a.head_dim) store_out(a, (const T*)nullptr, row, head, lane + 64 * e, o[e]);
 }
 
-template <typename T, int DP>
-int launch_prefill_dp(const PagedAttnArgs& a, dim3 grid, hipStream_t st) {
-    const dim3 block(kPreWaves * 64);
-    const uint32_t lds = 2 * PreShape<T, DP>::BYTES;
+template <typename T, int DP, int RW>
+int launch_prefill_rw(const PagedAttnArgs& a, hipStream_t st) {
+    const dim3 block(kPreWaves * 64), grid((unsigned)((long long)a.n_tiles * a.kv_heads * a.n_splits));
+    const uint32_t lds = PreShape<T, DP, RW>::LDS;
     const bool cap = a.sc.softcap > 0.0f, bias = a.sc.slopes != nullptr;
     const auto go = [&](auto kernel) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
@@ -488,28 +530,37 @@ int launch_prefill_dp(const PagedAttnArgs& a, dim3 grid, hipStream_t st) {
         launch_k(kernel, grid, block, lds, st, a);
         return UOCR_HIP_OK;
     };
-    if (cap && bias) return go(paged_prefill_kernel<T, DP, true, true>);
-    if (cap) return go(paged_prefill_kernel<T, DP, true, false>);
-    if (bias) return go(paged_prefill_kernel<T, DP, false, true>);
-    return go(paged_prefill_kernel<T, DP, false, false>);
+    if (cap && bias) return go(paged_prefill_kernel<T, DP, true, true, RW>);
+    if (cap) return go(paged_prefill_kernel<T, DP, true, false, RW>);
+    if (bias) return go(paged_prefill_kernel<T, DP, false, true, RW>);
+    return go(paged_prefill_kernel<T, DP, false, false, RW>);
+}
+template <typename T, int DP>
+int launch_prefill_dp(const PagedAttnArgs& a, int rw, hipStream_t st) {
+    if constexpr (DP <= 128) {
+        if constexpr (sizeof(T) == 4)
+            if (rw == 1) return launch_prefill_rw<T, DP, 1>(a, st);
+        if (rw == 2) return launch_prefill_rw<T, DP, 2>(a, st);
+    }
+    return launch_prefill_rw<T, DP, 4>(a, st);
 }
 
 template <typename T>
-int launch_prefill_t(const PagedAttnArgs& a, dim3 grid, hipStream_t st) {
+int launch_prefill_t(const PagedAttnArgs& a, int rw, hipStream_t st) {
     int rc;
-    if (a.head_dim <= 64) rc = launch_prefill_dp<T, 64>(a, grid, st);
-    else if (a.head_dim <= 96) rc = launch_prefill_dp<T, 96>(a, grid, st);
-    else if (a.head_dim <= 128) rc = launch_prefill_dp<T, 128>(a, grid, st);
-    else if (a.head_dim <= 192) rc = launch_prefill_dp<T, 192>(a, grid, st);
-    else rc = launch_prefill_dp<T, 256>(a, grid, st);
+    if (a.head_dim <= 64) rc = launch_prefill_dp<T, 64>(a, rw, st);
+    else if (a.head_dim <= 96) rc = launch_prefill_dp<T, 96>(a, rw, st);
+    else if (a.head_dim <= 128) rc = launch_prefill_dp<T, 128>(a, rw, st);
+    else if (a.head_dim <= 192) rc = launch_prefill_dp<T, 192>(a, rw, st);
+    else rc = launch_prefill_dp<T, 256>(a, rw, st);
     if (rc) return rc;
     if (a.n_splits > 1)
         launch_k(paged_prefill_join_kernel<T>, dim3((unsigned)(((long long)a.rows * a.heads + 3) / 4)), dim3(256), 0, st, a);
     return UOCR_HIP_OK;
 }
 
-int launch_prefill_f32(const PagedAttnArgs& a, dim3 grid, hipStream_t st);
-int launch_prefill_bf16(const PagedAttnArgs& a, dim3 grid, hipStream_t st);
-int launch_prefill_f16(const PagedAttnArgs& a, dim3 grid, hipStream_t st);
+int launch_prefill_f32(const PagedAttnArgs& a, int rw, hipStream_t st);
+int launch_prefill_bf16(const PagedAttnArgs& a, int rw, hipStream_t st);
+int launch_prefill_f16(const PagedAttnArgs& a, int rw, hipStream_t st);
 
 }  // namespace uocr_hip

@@ -3,6 +3,6 @@
 
 namespace uocr_hip {
 
-int launch_prefill_f16(const PagedAttnArgs& a, dim3 grid, hipStream_t st) { return launch_prefill_t<f16>(a, grid, st); }
+int launch_prefill_f16(const PagedAttnArgs& a, int rw, hipStream_t st) { return launch_prefill_t<f16>(a, rw, st); }
 
 }  // namespace uocr_hip

@@ -3,6 +3,6 @@
 
 namespace uocr_hip {
 
-int launch_prefill_f32(const PagedAttnArgs& a, dim3 grid, hipStream_t st) { return launch_prefill_t<float>(a, grid, st); }
+int launch_prefill_f32(const PagedAttnArgs& a, int rw, hipStream_t st) { return launch_prefill_t<float>(a, rw, st); }
 
 }  // namespace uocr_hip
