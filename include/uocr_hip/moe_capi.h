@@ -568,7 +568,7 @@ int uocr_hip_rope_append_paged(const uocr_hip_rows* q, const uocr_hip_rows* k, c
  * What is not seen has no influence, whatever its values (NaN and infinities included). */
 typedef struct {
     int heads;             /* query heads, a multiple of the cache's kv_heads */
-    float scale;           /* 0: 1 / sqrt(head_dim) */
+    float scale;           /* 0: 1 / sqrt(head_dim); else of magnitude 1e-15 .. 1e15, as is softcap */
     float softcap;         /* 0: none */
     const float* slopes;   /* [heads] f32 or NULL */
     int causal;            /* prefill only (a single new token sees no later key) */

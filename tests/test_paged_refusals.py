@@ -68,7 +68,7 @@ def test_caches(kw, code):
 @pytest.mark.parametrize("kw,code", [
     (dict(o=opts(heads=0)), EINVAL), (dict(o=opts(heads=3)), EINVAL), (dict(o=opts(heads=-2)), EINVAL),
     (dict(o=opts(scale=float("nan"))), EINVAL), (dict(o=opts(scale=float("inf"))), EINVAL), (dict(o=opts(softcap=-1.0)), EINVAL),
-    (dict(o=opts(softcap=float("nan"))), EINVAL), (dict(o=opts(window=-1)), EINVAL), (dict(batch=-1), EINVAL),
+    (dict(o=opts(softcap=float("nan"))), EINVAL), (dict(o=opts(softcap=1e-30)), EUNSUPPORTED), (dict(o=opts(scale=1e30)), EUNSUPPORTED), (dict(o=opts(window=-1)), EINVAL), (dict(batch=-1), EINVAL),
     (dict(hint=-1), EINVAL), (dict(q=rows(data=None)), EINVAL), (dict(out=rows(data=None)), EINVAL),
     (dict(q=rows(dtype=0)), EINVAL), (dict(q=rows(dtype=3)), EINVAL), (dict(out=rows(dtype=2)), EINVAL),
     (dict(q=rows(data=A + 4)), EUNSUPPORTED), (dict(q=rows(row_stride=513)), EUNSUPPORTED),

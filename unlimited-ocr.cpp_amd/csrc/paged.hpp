@@ -19,7 +19,7 @@ constexpr int kPagedCounters = 16384;   // (sequence, KV head, 16 query heads) o
 constexpr int kPagedMagic = 0x70616765; // first word of a workspace that was set up
 constexpr int kPagedHead = 64 + kPagedCounters * 4;  // bytes before a workspace's partial results
 constexpr int kPagedUnitTiles = 8;     // tiles of keys that one workgroup takes alone
-constexpr int kPagedPrefillTarget = 512;  // workgroups that a split prefill call aims at
+constexpr int kPagedPrefillTarget = 1024;  // workgroups of a split prefill call at most
 constexpr int kPagedMaxSplits = 128;
 
 // n / d for 0 <= n < 2^31 by a multiplication: with s = ceil(log2 d) and
@@ -141,7 +141,8 @@ inline DecodePlan paged_decode_plan(long long batch, int heads, int kv_heads, in
 // How a prefill call is shared out: workgroups of 4 waves, `row_waves` of them along the (row, head)
 // pairs of a KV head (32 each), the others on other tiles of keys; `tiles` of pairs per KV head at
 // most (each entry rounds up by less than one); the keys split over `splits` workgroups where
-// those leave most of the chip idle, 256 keys in each at least.
+// those leave some of the chip idle, 256 keys in each at least (64 rows of 32 heads on 16000 keys: 1 split 351 us,
+// 3 129, 12 61; 1024 rows of 16 heads of 256: 1 69, 2 56, 3 65).
 // 128 pairs per workgroup share K and V best, 64 or 32 leave fewer rounds one after the other and more
 // workgroups: they are for calls that do not fill the chip, and need keys for every wave. us with 4 / 2 / 1 row
 // waves, head_dim 128 (workgroups of 128 pairs):
@@ -165,10 +166,21 @@ inline PrefillPlan paged_prefill_plan(long long rows, long long batch, int heads
         else if (groups(4) < (f32 ? 1024 : 512) && max_keys > (f32 ? 32 : 64)) p.row_waves = 2;
     }
     p.tiles = tiles(p.row_waves);
-    const long long units = groups(p.row_waves), want = kPagedPrefillTarget / units, most = max_keys / 256;
-    long long n = want < most ? want : most;
-    if (n > kPagedMaxSplits) n = kPagedMaxSplits;
-    p.splits = n < 1 ? 1 : (int)n;
+    // Splits: the fewest rounds of tiles one after the other, with 4 tiles' time for a workgroup's
+    // beginning and end and for the join. `units`: the workgroups there are likely to be.
+    const long long slots = head_dim > 128 || p.row_waves == 1 ? 256 : 512;
+    long long per_kv = batch == 1 ? (pairs + 32 * p.row_waves - 1) / (32 * p.row_waves) : pairs / (32 * p.row_waves) + (batch + 1) / 2;
+    if (per_kv < batch) per_kv = batch;
+    const long long units = per_kv * kv_heads, keys = f32 ? 32 : 64, most = max_keys / 256;
+    if (units >= slots) return p;
+    long long best = 1ll << 62;
+    for (long long n = 1; n <= kPagedMaxSplits && (n == 1 || (n <= most && units * n <= kPagedPrefillTarget)); ++n) {
+        const long long rounds = (units * n + slots - 1) / slots, cost = rounds * (4 * max_keys / (keys * n) + 16) + (n > 1 ? 16 + n : 0);
+        if (cost < best) {
+            best = cost;
+            p.splits = (int)n;
+        }
+    }
     return p;
 }
 

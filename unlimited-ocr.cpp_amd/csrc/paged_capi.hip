@@ -80,6 +80,9 @@ int attn_args(const uocr_hip_paged_cache* cache, const uocr_hip_attention_opts* 
         return set_error(UOCR_HIP_EINVAL, "attention: rows, batch and max_kv_len must be >= 0");
     if (!std::isfinite(o->scale) || !std::isfinite(o->softcap) || o->softcap < 0.0f)
         return set_error(UOCR_HIP_EINVAL, "attention: scale and softcap must be finite, softcap >= 0");
+    if ((o->scale != 0.0f && !(std::fabs(o->scale) >= 1e-15f && std::fabs(o->scale) <= 1e15f)) ||
+        (o->softcap != 0.0f && !(o->softcap >= 1e-15f && o->softcap <= 1e15f)))
+        return set_error(UOCR_HIP_EUNSUPPORTED, "attention: |scale| and softcap, if not 0, must be in [1e-15, 1e15]");
     if (o->window < 0) return set_error(UOCR_HIP_EINVAL, "attention: window must be >= 0");
     if ((long long)rows * o->heads > INT_MAX)
         return set_error(UOCR_HIP_EUNSUPPORTED, "attention: more than 2^31 - 1 (row, head) pairs");
@@ -102,7 +105,10 @@ int attn_args(const uocr_hip_paged_cache* cache, const uocr_hip_attention_opts* 
     a->group = o->heads / cache->kv_heads;
     a->seqs = d_seqs;
     a->kv_len = d_kv_len;
-    a->sc = PagedScores{o->scale != 0.0f ? o->scale : 1.0f / sqrtf((float)cache->head_dim), o->softcap, o->slopes};
+    const double log2e = 1.4426950408889634, scale = o->scale != 0.0f ? o->scale : 1.0 / std::sqrt((double)cache->head_dim);
+    const double in = o->softcap > 0.0f ? scale / o->softcap : 0.0;
+    a->sc = PagedScores{(float)(scale * log2e), (float)(o->softcap * log2e), (float)in, (float)(2.0 * log2e * in), o->slopes,
+                        scale < 0.0};
     a->mask = MaskArgs{o->causal != 0, o->window, o->prefix_both_ways != 0, o->prefix_len, o->key_begin, o->key_end};
     return UOCR_HIP_OK;
 }

@@ -197,7 +197,7 @@ struct DecodeWave {
         load_v(a, at < 0 ? 0 : at, vw);
         for (int t = t_begin; t < t_end; t += step) {
             const uint32_t seen = (uint32_t)__ballot(in) & kAll, lost = (uint32_t)__ballot(at < 0) & kAll;
-            const int dist0 = r.len - 1 - base;
+            const float dist0 = (float)(r.len - 1 - base);
             const bool more = t + step < t_end;
             if (more) place(t + step);
             // scores: keys h * 16 + g * 4 + i of head col
@@ -225,7 +225,7 @@ struct DecodeWave {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int key = h * 16 + g * 4 + i;
-                    float x = score2<CAP, BIAS, F32>(s[h][i], a.sc, slope2, dist0 - key);
+                    float x = score2<CAP, BIAS, F32>(s[h][i], a.sc, slope2, dist0 - (float)key);
                     if (lost >> key & 1) x = NAN;
                     p[h][i] = seen >> key & 1 ? x : -INFINITY;
                     top = fmaxf(top, p[h][i]);
@@ -667,7 +667,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_decode_join_kernel(PagedAt
 template <typename T, int DP>
 void launch_dp(const PagedAttnArgs& a, hipStream_t st) {
     const int kvb = a.kv_heads * ((a.group + kDecCols - 1) / kDecCols);
-    const bool cap = a.sc.softcap > 0.0f, bias = a.sc.slopes != nullptr;
+    const bool cap = a.sc.cap2 > 0.0f, bias = a.sc.slopes != nullptr;
     const dim3 block(kDecWaves<DP> * 64);
     // (the join takes 16 bytes per thread)
     const uint32_t lds = std::max<uint32_t>(kDecWaves<DP> * std::min(a.group, kDecCols) * (DP + 4) * sizeof(float), block.x * 16);

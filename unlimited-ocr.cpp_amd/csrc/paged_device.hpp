@@ -19,10 +19,13 @@ struct PagedRows {
     long long row_bytes, head_bytes;
 };
 
+// Scores in units of log 2 (the softmax runs on exp2), with log2(e) folded into the constants
 struct PagedScores {
-    float scale;          // applied to q.k
-    float softcap;        // 0: none
+    float scale2;   // scale log2(e)
+    float cap2;     // softcap log2(e); 0: no cap
+    float in, in2;  // scale / softcap, and 2 log2(e) of that
     const float* slopes;  // [heads] or null
+    int negative;   // scale < 0
 };
 
 struct PagedAttnArgs {
@@ -80,22 +83,15 @@ __device__ __forceinline__ long long shfl64(long long v, int src) {
     return (long long)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo);
 }
 
-// Score of a visible pair in units of log 2 (the softmax runs on exp2).
+// Score of a visible pair; dist: positions between query and key (for the bias)
 template <bool CAP, bool BIAS, bool EXACT>
-__device__ __forceinline__ float score2(float qk, const PagedScores& sc, float slope2, int dist) {
-    float s = qk * sc.scale;
-    if constexpr (CAP) {
-        const float x = s / sc.softcap;
-        if constexpr (EXACT) {
-            s = sc.softcap * tanhf(x);
-        } else {
-            // 1 - 2 / (e^2|x| + 1): absolute error below 2^-22, a step of f16 scores of 1024
-            const float e = __builtin_amdgcn_exp2f(fabsf(x) * (2.0f * kLog2e));
-            s = copysignf(sc.softcap * fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f), x);
-        }
-    }
-    s *= kLog2e;
-    if constexpr (BIAS) s = fmaf(-slope2, (float)(dist < 0 ? -dist : dist), s);
+__device__ __forceinline__ float score2(float qk, const PagedScores& sc, float slope2, float dist) {
+    float s;
+    if constexpr (!CAP) s = qk * sc.scale2;
+    else if constexpr (EXACT) s = sc.cap2 * tanhf(qk * sc.in);
+    // tanh x = 1 - 2 / (e^2x + 1): absolute error below 2^-22, a step of f16 scores of 1024
+    else s = fmaf(-2.0f * sc.cap2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(qk * sc.in2) + 1.0f), sc.cap2);
+    if constexpr (BIAS) s = fmaf(-slope2, fabsf(dist), s);
     return s;
 }
 
@@ -140,8 +136,8 @@ __device__ void row_attention(const PagedAttnArgs& a, int seq, int row, int head
                 const T* k = reinterpret_cast<const T*>(kbase + off);
                 float x = 0.0f;
                 for (int d = 0; d < D; ++d) x = fmaf((float)q[d], (float)k[d], x);
-                const int dist = pos - j;
-                s = a.sc.softcap > 0.0f ? score2<true, true, true>(x, a.sc, slope2, dist)
+                const float dist = (float)(pos - j);
+                s = a.sc.cap2 > 0.0f ? score2<true, true, true>(x, a.sc, slope2, dist)
                                         : score2<false, true, true>(x, a.sc, slope2, dist);
             }
         }

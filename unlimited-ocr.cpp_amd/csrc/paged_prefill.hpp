@@ -188,7 +188,7 @@ __global__ __launch_bounds__(kPreWaves * 64, (PreShape<T, DP, RW>::RESIDENT)) vo
     {
         const char* qp = a.q.p + row * a.q.row_bytes + head * a.q.head_bytes;
         // a negative scale is moved into q: the maximum is taken before the scale
-        const uint32_t flip = a.sc.scale < 0.0f ? (F32 ? 0x80000000u : 0x80008000u) : 0u;
+        const uint32_t flip = a.sc.negative ? (F32 ? 0x80000000u : 0x80008000u) : 0u;
 #pragma unroll
         for (int f = 0; f < NF; ++f) {
             const int d = (2 * f + h) * (16 / ES);
@@ -201,8 +201,10 @@ __global__ __launch_bounds__(kPreWaves * 64, (PreShape<T, DP, RW>::RESIDENT)) vo
         }
     }
     PagedScores sc = a.sc;
-    sc.scale = fabsf(sc.scale);
-    const float scale2 = sc.scale * kLog2e;
+    sc.scale2 = fabsf(sc.scale2);
+    sc.in = fabsf(sc.in);
+    sc.in2 = fabsf(sc.in2);
+    const float scale2 = sc.scale2;
     float slope2 = 0.0f;
     if constexpr (BIAS) slope2 = a.sc.slopes[head] * kLog2e;
 
@@ -279,12 +281,12 @@ __global__ __launch_bounds__(kPreWaves * 64, (PreShape<T, DP, RW>::RESIDENT)) vo
                     }
                 const bool whole = __all((seen & kAll) == kAll);
                 if constexpr (CAP || BIAS) {
-                    const int dist0 = pos - base - 4 * h;
+                    const float dist0 = (float)(pos - base - 4 * h);
 #pragma unroll
                     for (int b = 0; b < KB; ++b)
 #pragma unroll
                         for (int r = 0; r < 16; ++r)
-                            s[b][r] = score2<CAP, BIAS, F32>(s[b][r], sc, slope2, dist0 - (b * 32 + 8 * (r >> 2) + (r & 3)));
+                            s[b][r] = score2<CAP, BIAS, F32>(s[b][r], sc, slope2, dist0 - (float)(b * 32 + 8 * (r >> 2) + (r & 3)));
                 }
                 constexpr bool kScaled = CAP || BIAS;
                 if (!whole) {
@@ -521,7 +523,7 @@ template <typename T, int DP, int RW>
 int launch_prefill_rw(const PagedAttnArgs& a, hipStream_t st) {
     const dim3 block(kPreWaves * 64), grid((unsigned)((long long)a.n_tiles * a.kv_heads * a.n_splits));
     const uint32_t lds = PreShape<T, DP, RW>::LDS;
-    const bool cap = a.sc.softcap > 0.0f, bias = a.sc.slopes != nullptr;
+    const bool cap = a.sc.cap2 > 0.0f, bias = a.sc.slopes != nullptr;
     const auto go = [&](auto kernel) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
