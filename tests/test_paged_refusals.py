@@ -163,16 +163,6 @@ def test_frequencies():
     assert (np.diff(h / f.astype(np.float32)) <= 1e-6).all()
 
 
-def test_packed_structs():
-    a = RowsC(A + 16, 2, 2**40, 3)
-    b = AttentionOptsC(32, 0.5, 30.0, A, 1, 77, 2 * A, 1, 3 * A, 4 * A)
-    assert _lib.ROWS_PACK(A + 16, 2, 2**40, 3) == bytes(a)
-    packed = _lib.OPTS_PACK(32, 0.5, 30.0, A, True, 77, 2 * A, True, 3 * A, 4 * A)
-    again = AttentionOptsC.from_buffer_copy(packed)
-    assert len(packed) == C.sizeof(AttentionOptsC)
-    assert all(getattr(again, n) == getattr(b, n) for n, _ in AttentionOptsC._fields_)
-
-
 def test_python_refuses_before_the_library():
     torch = pytest.importorskip("torch")
     from uocr_hip import paged
@@ -189,6 +179,10 @@ def test_python_refuses_before_the_library():
     q = torch.zeros(2, 4, 64)
     with pytest.raises(ValueError, match="GPU"):
         paged.rope(q, None, t[0, :2], torch.zeros(32), q, None)
+    with pytest.raises(TypeError, match="tensor"):
+        paged._n.rope([], None, None, None, None, None, 0, 1.0, 0)
+    with pytest.raises(TypeError, match="9 arguments"):
+        paged._n.rope(q)
     with pytest.raises(ValueError, match="scaling"):
         paged.rope_frequencies(64, scaling="dynamic")
     f, m = paged.rope_frequencies(64, scaling="parts", factor_len=8.0, original_len=4096)

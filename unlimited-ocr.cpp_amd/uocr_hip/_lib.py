@@ -1,7 +1,6 @@
 """ctypes loader and signatures for libuocr_hip.so."""
 import ctypes as C
 import os
-import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # UOCR_HIP_LIB overrides the in-tree library (used to compare builds)
@@ -75,11 +74,6 @@ class AttentionOptsC(C.Structure):
     _fields_ = [("heads", C.c_int), ("scale", C.c_float), ("softcap", C.c_float), ("slopes", C.c_void_p),
                 ("causal", C.c_int), ("window", C.c_int), ("prefix_len", C.c_void_p), ("prefix_both_ways", C.c_int),
                 ("key_begin", C.c_void_p), ("key_end", C.c_void_p)]
-
-
-# RowsC and AttentionOptsC as bytes, for calls that pass them by address (a third of a Structure's time)
-ROWS_PACK = struct.Struct("@Piqq").pack
-OPTS_PACK = struct.Struct("@iffPiiPiPP").pack
 
 
 def lib_path():

@@ -5,58 +5,46 @@ the tensors' device). Tensors a call works on belong to one device and stay
 alive, and unchanged by others, until the stream has run it.
 """
 import ctypes as C
+import importlib.machinery
+import importlib.util
+import os
 
 import torch
 
 from . import _lib
-from ._lib import OPTS_PACK, ROWS_PACK, PagedCacheC, check, load
+from ._lib import PagedCacheC, check, load
 
 _DTYPE = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 SCALING = {"none": 0, "linear": 1, "base": 2, "parts": 3}
 
 
-# The checks below run before every launch, which takes a few us itself: each reads
-# a tensor's attributes once, and builds a message only to raise it.
-
-def _rows(t, name, shape, index):
-    """uocr_hip_rows of a tensor [rows, heads, head_dim] on GPU `index` whose last dim is contiguous."""
-    st = t.stride()
-    if t.shape != shape or (st[2] != 1 and shape[2] > 1):
-        raise ValueError(f"{name} must be [rows, heads, head_dim] = {tuple(shape)} with contiguous dims of a head, got "
-                         f"{tuple(t.shape)} with strides {tuple(st)}")
-    if t.get_device() != index:
-        raise ValueError(f"{name} is on {t.device}, not on GPU {index}")
-    dt = _DTYPE.get(t.dtype)
-    if dt is None:
-        raise TypeError(f"{name} must be f32, bf16 or f16")
-    return ROWS_PACK(t.data_ptr(), dt, st[0], st[1])
+def _native():
+    """The native binding (csrc/torch_binding.cpp), on the entry points of the loaded library."""
+    lib = load()
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "lib", "_uocr_torch.so")
+    if not os.path.exists(path):
+        raise FileNotFoundError(f"{path} is missing: build it first (python -c 'import __graft_entry__ as g; g.build()')")
+    spec = importlib.util.spec_from_file_location("_uocr_torch", path,
+                                                  loader=importlib.machinery.ExtensionFileLoader("_uocr_torch", path))
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    m.bind(*(C.cast(getattr(lib, "uocr_hip_" + n), C.c_void_p).value
+             for n in ("rope", "rope_append_paged", "paged_attention_decode", "paged_attention_prefill")))
+    return m
 
 
-def _shape(t, name, index):
-    """[rows, heads, head_dim] of a call's first tensor."""
-    if index < 0:
-        raise ValueError("tensors must be on a GPU")
-    shape = t.shape
-    if len(shape) != 3:
-        raise ValueError(f"{name} must be [rows, heads, head_dim], got {tuple(shape)}")
-    return shape
+_n = _native()
+_current_device = torch.cuda.current_device
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _vector(t, name, n, index, dtype=torch.int32):
-    """Device address of a contiguous vector of n entries (None: 0)."""
-    if t is None:
-        return 0
-    if t.dtype is not dtype or t.get_device() != index or t.numel() != n or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor of {n} entries on GPU {index}")
-    return t.data_ptr()
-
-
-def _call(fn, index, stream, *args):
+def _call(fn, index, stream, args):
     """fn(*args, stream) with GPU `index` current."""
-    if torch.cuda.current_device() != index:
+    if index >= 0 and _current_device() != index:
         with torch.cuda.device(index):
-            return _call(fn, index, stream, *args)
-    rc = fn(*args, torch._C._cuda_getCurrentRawStream(index) if stream is None else stream)
+            rc = fn(*args, _raw_stream(index) if stream is None else stream)
+    else:
+        rc = fn(*args, stream if stream is not None or index < 0 else _raw_stream(index))
     if rc:
         check(rc)
 
@@ -109,38 +97,15 @@ class PagedKVCache:
 def rope(q, k, positions, inv_freq, q_out, k_out, interleaved=False, factor=1.0, stream=None):
     """q_out, k_out = q, k [rows, heads, head_dim] with the first 2 * len(inv_freq) dims of every
     head turned by positions[row] * inv_freq[i]. k and k_out may be None; q_out may be q, k_out k."""
-    g = q.get_device()
-    shape = _shape(q, "q", g)
-    n, h, d = shape
-    if (k is None) != (k_out is None):
-        raise ValueError("k and k_out go together")
-    hk, ki, ko = 0, None, None
-    if k is not None:
-        ks = _shape(k, "k", g)
-        hk = ks[1]
-        ks = torch.Size((n, hk, d))
-        ki, ko = _rows(k, "k", ks, g), _rows(k_out, "k_out", ks, g)
-    half = inv_freq.numel()
-    _call(load().uocr_hip_rope, g, stream, _rows(q, "q", shape, g), ki, n, h, hk, d, _vector(positions, "positions", n, g),
-          _vector(inv_freq, "inv_freq", half, g, torch.float32), 2 * half, interleaved, factor,
-          _rows(q_out, "q_out", shape, g), ko)
+    _call(_n.rope, q.get_device(), stream, (q, k, positions, inv_freq, q_out, k_out, interleaved, factor))
 
 
 def rope_append(q, k, v, positions, inv_freq, cache, seqs, rows, q_out, interleaved=False, factor=1.0, stream=None):
     """rope() of q into q_out, and of k with v into the cache: row t becomes row rows[t] of sequence
     seqs[t] (outside the table's sequences: padding, left alone). q_out has the cache's
     type; inv_freq None (or empty) appends without rotation."""
-    g = cache.index
-    shape = _shape(q, "q", g)
-    n, h, d = shape
-    ks = torch.Size((n, cache.kv_heads, cache.head_dim))
-    half = inv_freq.numel() if inv_freq is not None else 0
-    if d != cache.head_dim:
-        raise ValueError(f"q has head_dim {d}, the cache {cache.head_dim}")
-    _call(load().uocr_hip_rope_append_paged, g, stream, _rows(q, "q", shape, g), _rows(k, "k", ks, g), _rows(v, "v", ks, g),
-          n, h, _vector(positions, "positions", n, g) if half else 0,
-          _vector(inv_freq, "inv_freq", half, g, torch.float32) if half else 0, 2 * half, interleaved, factor,
-          cache.address, _vector(seqs, "seqs", n, g), _vector(rows, "rows", n, g), _rows(q_out, "q_out", shape, g))
+    _call(_n.rope_append, cache.index, stream,
+          (q, k, v, positions, inv_freq, cache.address, cache.index, seqs, rows, q_out, interleaved, factor))
 
 
 def attention_workspace(cache, heads, rows):
@@ -151,28 +116,8 @@ def attention_workspace(cache, heads, rows):
         raise _lib.HipError(_lib.EINVAL, load().uocr_hip_last_error().decode())
     ws = torch.empty(n, dtype=torch.uint8, device=cache.device)
     if n:
-        _call(load().uocr_hip_paged_attention_workspace_init, cache.index, None, ws.data_ptr(), n)
+        _call(load().uocr_hip_paged_attention_workspace_init, cache.index, None, (ws.data_ptr(), n))
     return ws
-
-
-def _attention(fn, cache, q, out, kv_len, seqs, batch, scale, softcap, slopes, causal, window, prefix_len, both_ways, key_begin,
-               key_end, max_kv_len, workspace, stream, *rows):
-    g = cache.index
-    shape = _shape(q, "q", g)
-    n, h, d = shape
-    if d != cache.head_dim:
-        raise ValueError(f"q has head_dim {d}, the cache {cache.head_dim}")
-    s = cache.n_seqs
-    opts = OPTS_PACK(h, scale or 0.0, softcap, _vector(slopes, "slopes", h, g, torch.float32), causal, window,
-                     _vector(prefix_len, "prefix_len", s, g), both_ways, _vector(key_begin, "key_begin", n, g),
-                     _vector(key_end, "key_end", n, g))
-    ws = size = 0
-    if workspace is not None:
-        ws, size = workspace.data_ptr(), workspace.nbytes
-        if workspace.get_device() != g or not workspace.is_contiguous():
-            raise ValueError(f"workspace must be a contiguous tensor on GPU {g}")
-    _call(fn, g, stream, cache.address, opts, _rows(q, "q", shape, g), *rows, _vector(seqs, "seqs", batch, g),
-          _vector(kv_len, "kv_len", s, g), max_kv_len, _rows(out, "out", shape, g), ws, size)
 
 
 def attention_decode(q, cache, kv_len, out, seqs=None, scale=None, softcap=0.0, slopes=None, window=0, prefix_len=None,
@@ -181,9 +126,9 @@ def attention_decode(q, cache, kv_len, out, seqs=None, scale=None, softcap=0.0, 
     last position of sequence seqs[b] (b if None), its K and V in the cache already. kv_len and
     prefix_len [n_seqs] int32; see uocr_hip_attention_opts for the scores and masks.
     max_kv_len (0: the table's room) only chooses the split."""
-    n = q.size(0)
-    _attention(load().uocr_hip_paged_attention_decode, cache, q, out, kv_len, seqs, n, scale, softcap, slopes, True, window,
-               prefix_len, False, key_begin, key_end, max_kv_len, workspace, stream, n)
+    _call(_n.attention, cache.index, stream,
+          (q, cache.address, cache.index, None, kv_len, out, seqs, True, scale, softcap, slopes, window, prefix_len, False,
+           key_begin, key_end, max_kv_len, workspace))
 
 
 def attention_prefill(q, cache, q_start, kv_len, out, seqs=None, causal=True, scale=None, softcap=0.0, slopes=None, window=0,
@@ -191,9 +136,8 @@ def attention_prefill(q, cache, q_start, kv_len, out, seqs=None, causal=True, sc
                       workspace=None, stream=None):
     """Attention of many rows per sequence: rows q_start[b] .. q_start[b + 1] - 1 of q and out
     [rows, heads, head_dim] are the last positions of sequence seqs[b] (b if None). See attention_decode."""
-    batch = q_start.numel() - 1
-    if batch < 0:
-        raise ValueError("q_start needs batch + 1 entries")
-    _attention(load().uocr_hip_paged_attention_prefill, cache, q, out, kv_len, seqs, batch, scale, softcap, slopes, causal,
-               window, prefix_len, prefix_both_ways, key_begin, key_end, max_kv_len, workspace, stream, q.size(0), batch,
-               _vector(q_start, "q_start", batch + 1, cache.index))
+    if q_start is None:
+        raise ValueError("q_start is missing")
+    _call(_n.attention, cache.index, stream,
+          (q, cache.address, cache.index, q_start, kv_len, out, seqs, causal, scale, softcap, slopes, window, prefix_len,
+           prefix_both_ways, key_begin, key_end, max_kv_len, workspace))
