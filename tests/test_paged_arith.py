@@ -51,6 +51,28 @@ static int spans() {
             CHECK(found == n);
         }
     }
+    // rows first .. last together: every key that one of them sees is in a range, and none beyond the sequence
+    for (int causal = 0; causal < 2; ++causal)
+    for (int both = 0; both < 2; ++both)
+    for (int window : {0, 1, 2, 5, 9, M}) {
+        if (window && !causal) continue;
+        for (int len = 0; len < 12; ++len)
+        for (int first = -3; first < len; ++first)
+        for (int last = first; last < len; ++last)
+        for (int prefix : {-1, 0, 1, 3, 7, 20, M}) {
+            int l0, h0, l1, h1;
+            tile_range(causal, window, both, first, last, len, prefix, l0, h0, l1, h1);
+            CHECK(l0 >= 0 && l1 >= 0 && h0 <= len && h1 <= len && h0 >= 0 && h1 >= 0);
+            for (int j = 0; j < len; ++j) {
+                bool seen = false;
+                for (int p = first; p <= last; ++p) seen = seen || row_span(causal, window, both, p, len, prefix, 0, M).has(j);
+                const bool in = (j >= l0 && j < h0) || (j >= l1 && j < h1);
+                CHECK(!seen || in);
+                // and no key that none sees, but where prefix rows before the first position stand for the last's
+                CHECK(!in || seen || first < 0);
+            }
+        }
+    }
     // the far end of int
     const Span s = row_span(1, 100, 0, M - 1, M, 50, 0, M);
     CHECK(s.b0 == 0 && s.e0 == 50 && s.b1 == M - 100 && s.e1 == M);

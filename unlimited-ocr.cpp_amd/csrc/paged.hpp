@@ -97,6 +97,18 @@ UOCR_HD inline Span row_span(int causal, int window, int both_ways, int pos, int
     return s;
 }
 
+// The keys that rows at positions first .. last see together (no limits of their own), as two
+// ranges that may overlap; hi 0 or lo >= hi: empty.
+UOCR_HD inline void tile_range(int causal, int window, int both_ways, int first, int last, int len, int prefix, int& lo0,
+                               int& hi0, int& lo1, int& hi1) {
+    const int hi = causal ? imin(len, last + 1) : len;
+    lo0 = 0;
+    hi0 = imax(imin(both_ways ? len : hi, prefix), 0);
+    lo1 = window && first >= window ? first - window + 1 : 0;
+    hi1 = imax(hi, 0);
+    if (lo1 >= hi1) hi1 = 0;
+}
+
 // A row's span as tiles of W keys on W-aligned positions: the first tile that
 // holds a key of each interval, and how many there are. Neighbouring intervals may share a
 // tile; it is walked once for each, with that interval's keys.

@@ -53,15 +53,21 @@ struct PreShape {
 // Row range of sequence entry b in [0, rows]
 __device__ __forceinline__ int pre_start(const PagedAttnArgs& a, int b) { return imin(imax(a.q_start[b], 0), a.rows); }
 
-// Entry b and tile within it of tile index t (tiles of entry after entry); -1: none
+// Entry b, its sequence and cache length, and the tile within it, of tile index t (tiles of entry after
+// entry); -1: none. A lane holds an entry, so that nothing is loaded one after the other.
 template <int ROWS>
-__device__ __forceinline__ int pre_find(const PagedAttnArgs& a, int t, int& tile) {
+__device__ __forceinline__ int pre_find(const PagedAttnArgs& a, int t, int& tile, int& seq, int& kv) {
     const int lane = threadIdx.x & 63;
     int before = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
         const int b = b0 + lane;
-        int n = 0;
-        if (b < a.batch) n = (imax(pre_start(a, b + 1) - pre_start(a, b), 0) * a.group + ROWS - 1) / ROWS;
+        int n = 0, my_seq = -1, my_kv = 0;
+        if (b < a.batch) {
+            my_seq = a.seqs ? a.seqs[b] : b;
+            if ((uint32_t)my_seq < (uint32_t)a.c.n_seqs) my_kv = a.kv_len[my_seq];
+            else my_seq = -1;
+            n = (imax(pre_start(a, b + 1) - pre_start(a, b), 0) * a.group + ROWS - 1) / ROWS;
+        }
         int sum = n;
 #pragma unroll
         for (int x = 1; x < 64; x *= 2) {
@@ -71,10 +77,12 @@ __device__ __forceinline__ int pre_find(const PagedAttnArgs& a, int t, int& tile
         const uint64_t hit = __ballot(before + sum > t);
         if (hit) {
             const int src = __builtin_ctzll(hit);
-            tile = t - before - (__shfl(sum, src, 64) - __shfl(n, src, 64));
+            tile = t - before - (__builtin_amdgcn_readlane(sum, src) - __builtin_amdgcn_readlane(n, src));
+            seq = __builtin_amdgcn_readlane(my_seq, src);
+            kv = __builtin_amdgcn_readlane(my_kv, src);
             return b0 + src;
         }
-        before += __shfl(sum, 63, 64);
+        before += __builtin_amdgcn_readlane(sum, 63);
     }
     return -1;
 }
@@ -127,13 +135,10 @@ __global__ __launch_bounds__(kPreWaves * 64, (PreShape<T, DP, RW>::RESIDENT)) vo
     // numbers of heads share every XCD's evenly (runs of one head per XCD: 4096 rows of 10 heads 158 us, this way 113).
     const int per = a.n_tiles * a.kv_heads, split = blockIdx.x / per, item = blockIdx.x % per;
     const int kvh = item % a.kv_heads;
-    int tile;
-    const int entry = pre_find<P::ROWS>(a, a.n_tiles - 1 - item / a.kv_heads, tile);
-    if (entry < 0) return;
-    const int seq = a.seqs ? a.seqs[entry] : entry;
-    if ((uint32_t)seq >= (uint32_t)a.c.n_seqs) return;
+    int tile, seq, kv;
+    const int entry = pre_find<P::ROWS>(a, a.n_tiles - 1 - item / a.kv_heads, tile, seq, kv);
+    if (entry < 0 || seq < 0) return;
     const int start = pre_start(a, entry), n = imax(pre_start(a, entry + 1) - start, 0);
-    const int kv = a.kv_len[seq];
     const bool gone = kv > a.c.capacity();  // more keys than the table has room for
     const int len = gone ? 0 : imax(kv, 0);
 
@@ -142,12 +147,19 @@ __global__ __launch_bounds__(kPreWaves * 64, (PreShape<T, DP, RW>::RESIDENT)) vo
     const bool live = packed < n * a.group;
     const int token = packed / a.group, row = start + imin(token, n - 1), head = kvh * a.group + packed % a.group;
     const int pos = len - n + token;
+    const int prefix = a.mask.prefix_len ? a.mask.prefix_len[seq] : 0;
     Span span{0, 0, 0, 0};
     if (live)
-        span = row_span(a.mask.causal, a.mask.window, a.mask.both_ways, pos, len, a.mask.prefix_len ? a.mask.prefix_len[seq] : 0,
+        span = row_span(a.mask.causal, a.mask.window, a.mask.both_ways, pos, len, prefix,
                         a.mask.key_begin ? a.mask.key_begin[row] : 0, a.mask.key_end ? a.mask.key_end[row] : len);
-    // keys that some row sees: two ranges
-    {
+    // keys that some row sees: two ranges. Rows without limits of their own: the first and last
+    // row's say it (the window moves on with the row, and so does the end).
+    int lo0, hi0, lo1, hi1;
+    if (!a.mask.key_begin && !a.mask.key_end) {
+        const int last = imin((tile + 1) * P::ROWS, n * a.group) - 1;
+        tile_range(a.mask.causal, a.mask.window, a.mask.both_ways, len - n + tile * P::ROWS / a.group,
+                   len - n + last / a.group, len, prefix, lo0, hi0, lo1, hi1);
+    } else {
         constexpr int kFar = 0x7fffffff;
         const bool in0 = span.e0 > span.b0, in1 = span.e1 > span.b1;
         const int r0 = wave_min(in0 ? span.b0 : kFar), r1 = wave_max(in0 ? span.e0 : 0);
@@ -158,17 +170,23 @@ __global__ __launch_bounds__(kPreWaves * 64, (PreShape<T, DP, RW>::RESIDENT)) vo
             s_range[wave][2] = r2;
             s_range[wave][3] = r3;
         }
-        if (tid == 0) s_lost = 0;
-    }
-    __syncthreads();
-    int lo0 = s_range[0][0], hi0 = s_range[0][1], lo1 = s_range[0][2], hi1 = s_range[0][3];
+        __syncthreads();
+        lo0 = lo1 = kFar;
+        hi0 = hi1 = 0;
 #pragma unroll
-    for (int w = 1; w < kPreWaves; ++w) {
-        lo0 = imin(lo0, s_range[w][0]);
-        hi0 = imax(hi0, s_range[w][1]);
-        lo1 = imin(lo1, s_range[w][2]);
-        hi1 = imax(hi1, s_range[w][3]);
+        for (int w = 0; w < kPreWaves; ++w) {
+            lo0 = imin(lo0, s_range[w][0]);
+            hi0 = imax(hi0, s_range[w][1]);
+            lo1 = imin(lo1, s_range[w][2]);
+            hi1 = imax(hi1, s_range[w][3]);
+        }
+        lo0 = __builtin_amdgcn_readfirstlane(lo0);
+        hi0 = __builtin_amdgcn_readfirstlane(hi0);
+        lo1 = __builtin_amdgcn_readfirstlane(lo1);
+        hi1 = __builtin_amdgcn_readfirstlane(hi1);
     }
+    if (tid == 0) s_lost = 0;
+    bool lost = false;  // a key of this lane's tiles has no page
     // as tiles; one range where a tile would be in both
     int t0 = hi0 ? lo0 / BN : 0, n0 = hi0 ? (hi0 - 1) / BN + 1 - t0 : 0;
     int t1 = hi1 ? lo1 / BN : 0, n1 = hi1 ? (hi1 - 1) / BN + 1 - t1 : 0;
@@ -216,11 +234,8 @@ __global__ __launch_bounds__(kPreWaves * 64, (PreShape<T, DP, RW>::RESIDENT)) vo
     auto place = [&](int t) {  // of key `lane` (mod BN); keys outside the range: those at its ends
         const int lo = t < n0 ? lo0 : lo1, hi = t < n0 ? hi0 : hi1;
         long long off = a.c.offset(seq, imin(imax(tile_base(t) + (lane & (BN - 1)), lo), hi - 1));
-        if (off < 0) {
-            s_lost = 1;
-            off = 0;
-        }
-        return off;
+        lost |= off < 0;
+        return off < 0 ? 0 : off;
     };
     auto load = [&](long long off) {
 #pragma unroll
@@ -356,6 +371,8 @@ __global__ __launch_bounds__(kPreWaves * 64, (PreShape<T, DP, RW>::RESIDENT)) vo
             if (t + KW < t_end) store(own + (P::BUFS == 2 ? (round + 1 & 1) * P::TILE : 0));
         }
     }
+    __syncthreads();
+    if (lost) s_lost = 1;
     __syncthreads();
     // the groups' sums of the same rows, by halves
 #pragma unroll
