@@ -130,6 +130,18 @@ def test_rope_many_rows_and_none(dev):
     R.close(x[[0, 65536, 70000]], want, np.full(want.shape, 2.0**-20))
 
 
+def test_rope_more_rows_than_one_grid(dev):
+    """Beyond 2^22 rows a workgroup takes several: the same results at both ends."""
+    n = (1 << 22) + 300
+    freq, _ = paged().rope_frequencies(8)
+    x = torch.ones(n, 1, 8, dtype=torch.float16, device=dev)
+    pos = torch.arange(n, dtype=torch.int32, device=dev)
+    paged().rope(x, None, pos, freq.to(dev), x, None)
+    rows = [0, 299, 300, 1 << 22, n - 1]
+    want = R.turned(np.ones((len(rows), 1, 8)), rows, freq.numpy(), 8, False, 1.0)
+    R.close(x[rows], want, R.HALF["f16"] * np.abs(want) + 2.0**-20)
+
+
 # ---- attention of one new token ------------------------------------------------
 
 def run_decode(dev, rng, pool, heads, out_dtype=None, seqs=None, spread=1.5, strided=False, **kw):
@@ -220,7 +232,8 @@ def test_decode_split_f32_large_scores(dev):
 
 @pytest.mark.parametrize("heads,kv_heads,d,lens,hint", [
     (4, 1, 64, [9000], 0), (32, 2, 128, [2500, 2500, 1, 0, 40], 2500), (3, 3, 96, [1200] * 9, 0), (16, 1, 256, [1500, 700], 0),
-    (18, 1, 64, [800] * 40, 0), (2, 2, 128, [30] * 300, 2000)])
+    (18, 1, 64, [800] * 40, 0), (2, 2, 128, [30] * 300, 2000),
+    (1, 1, 64, [700] + [9] * 1100, 0)])
 def test_decode_shares(dev, heads, kv_heads, d, lens, hint):
     """Many shares of one sequence (joined by a kernel of its own), a few of each, several sequences in one; on one
     workspace in turn, so that each call leaves it as the next needs it."""

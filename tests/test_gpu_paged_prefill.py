@@ -128,6 +128,21 @@ def test_prefill_few_rows_on_a_long_cache(dev, dtype, rows, heads, kv_heads):
     run_prefill(dev, rng, pool, [rows, max(1, rows // 2)], heads, check=check, window=300, prefix_len=[500, 100])
 
 
+@pytest.mark.parametrize("dtype,rows,heads,kv_heads,d", [
+    ("bf16", 900, 72, 72, 64), ("f16", 1030, 130, 65, 32), ("f32", 2050, 66, 66, 32), ("bf16", 300, 12, 3, 200), ("f32", 300, 4, 2, 256)])
+@pytest.mark.parametrize("kw", [dict(), dict(window=200, prefix_len=[100, 40]), dict(docs=130, softcap=8.0), dict(causal=False)])
+def test_prefill_whole_chip(dev, dtype, rows, heads, kv_heads, d, kw):
+    """Enough workgroups of 128 (row, head) pairs for the chip, and heads above 128: over many tiles of keys."""
+    kw = dict(kw)
+    rng = np.random.default_rng(rows)
+    lens, q = [rows + 70, 150], [rows, 150]
+    pool = R.Pool(rng, lens, kv_heads, d // 8 * 8, 16, dtype, dev)
+    doc = kw.pop("docs", 0)
+    if doc:
+        kw["key_begin"] = [p // doc * doc for n, r in zip(lens, q) for p in range(n - r, n)]
+    run_prefill(dev, rng, pool, q, heads, check={0, 1, 63, 127, 128, rows // 2, rows - 1, rows, rows + 149}, **kw)
+
+
 def test_prefill_sequences_by_slot(dev):
     rng = np.random.default_rng(7)
     pool = R.Pool(rng, [40, 90, 10], 2, 64, 16, "bf16", dev)

@@ -700,7 +700,7 @@ int launch_paged_decode(PagedAttnArgs a, int dtype, long long max_keys, void* ws
     const DecodePlan p = paged_decode_plan(a.batch, a.heads, a.kv_heads, dtype == UOCR_HIP_DTYPE_F32 ? 16 : 32, max_keys,
                                            std::min<long long>(a.c.capacity(), INT_MAX));
     a.n_splits = p.shares;
-    if ((long long)a.batch * a.kv_heads * p.blocks > INT_MAX)
+    if ((long long)a.batch * a.kv_heads * p.blocks >= 1 << 23)  // (a launch has fewer than 2^32 threads)
         return set_error(UOCR_HIP_EUNSUPPORTED, "attention: batch too large");
     if (p.shares)
         if (int rc = paged_take_workspace(a, p.records, a.batch, ws, ws_bytes)) return rc;

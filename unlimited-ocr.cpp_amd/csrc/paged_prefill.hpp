@@ -26,6 +26,8 @@
 #pragma once
 #include <hip/hip_runtime.h>
 
+#include <atomic>
+
 #include "launch.hpp"
 #include "paged_device.hpp"
 #include "paged_host.hpp"
@@ -536,23 +538,31 @@ __global__ __launch_bounds__(256) void paged_prefill_join_kernel(PagedAttnArgs a
         if (lane + 64 * e < a.head_dim) store_out(a, (const T*)nullptr, row, head, lane + 64 * e, o[e]);
 }
 
+// A launch of more than the 64 KiB of LDS that a kernel has by default; asked for once per device
+template <auto KERNEL>
+int launch_lds(const PagedAttnArgs& a, dim3 grid, uint32_t lds, hipStream_t st) {
+    static std::atomic<uint64_t> ready{0};
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (e == hipSuccess && !(ready.load(std::memory_order_relaxed) & bit)) {
+        e = hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e == hipSuccess) ready.fetch_or(bit, std::memory_order_relaxed);
+    }
+    if (e != hipSuccess) return set_error(UOCR_HIP_EHIP, std::string("paged prefill LDS: ") + hipGetErrorString(e));
+    launch_k(KERNEL, grid, dim3(kPreWaves * 64), lds, st, a);
+    return UOCR_HIP_OK;
+}
+
 template <typename T, int DP, int RW>
 int launch_prefill_rw(const PagedAttnArgs& a, hipStream_t st) {
-    const dim3 block(kPreWaves * 64), grid((unsigned)((long long)a.n_tiles * a.kv_heads * a.n_splits));
+    const dim3 grid((unsigned)((long long)a.n_tiles * a.kv_heads * a.n_splits));
     const uint32_t lds = PreShape<T, DP, RW>::LDS;
     const bool cap = a.sc.cap2 > 0.0f, bias = a.sc.slopes != nullptr;
-    const auto go = [&](auto kernel) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-        if (e != hipSuccess)
-            return set_error(UOCR_HIP_EHIP, std::string("paged prefill LDS: ") + hipGetErrorString(e));
-        launch_k(kernel, grid, block, lds, st, a);
-        return UOCR_HIP_OK;
-    };
-    if (cap && bias) return go(paged_prefill_kernel<T, DP, true, true, RW>);
-    if (cap) return go(paged_prefill_kernel<T, DP, true, false, RW>);
-    if (bias) return go(paged_prefill_kernel<T, DP, false, true, RW>);
-    return go(paged_prefill_kernel<T, DP, false, false, RW>);
+    if (cap && bias) return launch_lds<paged_prefill_kernel<T, DP, true, true, RW>>(a, grid, lds, st);
+    if (cap) return launch_lds<paged_prefill_kernel<T, DP, true, false, RW>>(a, grid, lds, st);
+    if (bias) return launch_lds<paged_prefill_kernel<T, DP, false, true, RW>>(a, grid, lds, st);
+    return launch_lds<paged_prefill_kernel<T, DP, false, false, RW>>(a, grid, lds, st);
 }
 template <typename T, int DP>
 int launch_prefill_dp(const PagedAttnArgs& a, int rw, hipStream_t st) {

@@ -45,11 +45,10 @@ __device__ __forceinline__ void store_n(char* p, const float (&x)[N]) {
     __builtin_memcpy(N == 1 ? p : (char*)__builtin_assume_aligned(p, 16), t, N * sizeof(T));
 }
 
-// TI, TO: types in and out; N: elements per access (8, or 1 where alignment or sizes ask for it)
+// One row. TI, TO: types in and out; N: elements per access (8, or 1 where alignment or sizes ask for it)
 template <typename TI, typename TO, int N>
-__global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs a) {
-    __shared__ float s_cos[128], s_sin[128];
-    const int t = blockIdx.x, tid = threadIdx.x, half = a.rotary / 2, D = a.head_dim;
+__device__ __forceinline__ void rope_row(const RopeArgs& a, int t, float* s_cos, float* s_sin) {
+    const int tid = threadIdx.x, half = a.rotary / 2, D = a.head_dim;
     long long page = -1;
     if (a.append) {
         const int seq = a.seqs[t];
@@ -128,9 +127,18 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs a) {
     }
 }
 
+template <typename TI, typename TO, int N>
+__global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs a) {
+    __shared__ float s_cos[128], s_sin[128];
+    for (long long t = blockIdx.x; t < a.rows; t += gridDim.x) {
+        if (t != blockIdx.x) __syncthreads();  // (the last row's sines are read)
+        rope_row<TI, TO, N>(a, (int)t, s_cos, s_sin);
+    }
+}
+
 template <typename TI, typename TO>
 void launch_n(const RopeArgs& a, bool vec, hipStream_t st) {
-    const dim3 grid(a.rows), block(kRopeThreads);
+    const dim3 grid(std::min(a.rows, 1 << 22)), block(kRopeThreads);  // (a launch has fewer than 2^32 threads)
     if (vec) launch_k(rope_kernel<TI, TO, 8>, grid, block, 0, st, a);
     else launch_k(rope_kernel<TI, TO, 1>, grid, block, 0, st, a);
 }
