@@ -34,22 +34,25 @@
 
 namespace uocr_hip {
 
-constexpr int kPreWaves = 4;
-
-// RW: waves along the rows; the other 4 / RW groups of waves take other tiles of keys
-template <typename T, int DP, int RW>
+// RW: waves along the rows; KW groups of them take turns at the tiles of keys
+template <typename T, int DP, int RW, int KW>
 struct PreShape {
-    static constexpr int ES = sizeof(T), KW = kPreWaves / RW;
+    static constexpr int ES = sizeof(T), WAVES = RW * KW;
     static constexpr int ROWS = RW * 32;  // packed query rows per workgroup
-    static constexpr int KEYS = ES == 4 ? 32 : 64;  // per tile
+    static constexpr int KEYS = ES == 4 || WAVES == 8 ? 32 : 64;  // per tile
     static constexpr int KSTR = DP * ES + 16;
     static constexpr int VPAD = ES == 4 ? 32 : (DP * 2 % 256 == 64 || DP * 2 % 256 == 192) ? 0 : 64;
     static constexpr int VSTR = DP * ES + VPAD;
     static constexpr int TILE = KEYS * (KSTR + VSTR);
     static constexpr int BUFS = KW == 1 ? 2 : 1;
-    static constexpr int LDS = TILE * KW * BUFS;
-    // workgroups per CU that registers and LDS allow
-    static constexpr int RESIDENT = DP > 128 || KW == 4 ? 1 : 2;
+    // 8 waves: the query operand waits in LDS (heads of 256: 64 registers; in them 4096 rows of 16 heads take 301 us, not 219)
+    static constexpr bool QLDS = WAVES == 8;
+    static constexpr int QAT = TILE * KW * BUFS, TILES = QAT + (QLDS ? ROWS * KSTR : 0);
+    static constexpr int OUT = ROWS * (DP * 4 + 16);                                    // a workgroup's rows on their way out
+    static constexpr int SUMS = KW == 1 ? 0 : (DP / 32 * 4 + 1) * 1024 * (WAVES / 2);  // half the waves' sums
+    static constexpr int LDS = TILES > OUT ? (TILES > SUMS ? TILES : SUMS) : OUT > SUMS ? OUT : SUMS;
+    // waves per SIMD that registers and LDS allow
+    static constexpr int PER_SIMD = WAVES == 8 ? 2 : DP > 128 || KW == 4 ? 1 : 2;
 };
 
 // Row range of sequence entry b in [0, rows]
@@ -116,18 +119,18 @@ __device__ __forceinline__ s16x4 lds_tr(const char* p) {
         (__attribute__((address_space(3))) s16x4*)(__attribute__((address_space(3))) void*)(void*)p);
 }
 
-template <typename T, int DP, bool CAP, bool BIAS, int RW>
-__global__ __launch_bounds__(kPreWaves * 64, (PreShape<T, DP, RW>::RESIDENT)) void paged_prefill_kernel(PagedAttnArgs a) {
-    typedef PreShape<T, DP, RW> P;
+template <typename T, int DP, bool CAP, bool BIAS, int RW, int KW>
+__global__ __launch_bounds__(RW * KW * 64, (PreShape<T, DP, RW, KW>::PER_SIMD)) void paged_prefill_kernel(PagedAttnArgs a) {
+    typedef PreShape<T, DP, RW, KW> P;
     constexpr bool F32 = sizeof(T) == 4;
-    constexpr int ES = sizeof(T), BN = P::KEYS, KB = BN / 32, CH = DP * ES / 16, KW = P::KW, GT = RW * 64, NL = BN * CH / GT;
+    constexpr int ES = sizeof(T), BN = P::KEYS, KB = BN / 32, CH = DP * ES / 16, GT = RW * 64, NL = BN * CH / GT;
     static_assert(BN * CH % GT == 0, "whole 16-byte units per thread");
     constexpr int KSTR = P::KSTR, VSTR = P::VSTR;
     constexpr int NF = F32 ? DP / 8 : DP / 16;  // 16-byte pieces of a query row per lane
     constexpr int DB = DP / 32;
     typedef typename Vec8<T>::type vec_t;
     extern __shared__ __attribute__((aligned(16))) char s_buf[];  // tiles: K rows, then V rows
-    __shared__ int s_range[kPreWaves][4];
+    __shared__ int s_range[P::WAVES][4];
     __shared__ int s_lost;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 31, h = lane >> 5;
@@ -176,7 +179,7 @@ __global__ __launch_bounds__(kPreWaves * 64, (PreShape<T, DP, RW>::RESIDENT)) vo
         lo0 = lo1 = kFar;
         hi0 = hi1 = 0;
 #pragma unroll
-        for (int w = 0; w < kPreWaves; ++w) {
+        for (int w = 0; w < P::WAVES; ++w) {
             lo0 = imin(lo0, s_range[w][0]);
             hi0 = imax(hi0, s_range[w][1]);
             lo1 = imin(lo1, s_range[w][2]);
@@ -204,8 +207,9 @@ __global__ __launch_bounds__(kPreWaves * 64, (PreShape<T, DP, RW>::RESIDENT)) vo
     const int t_begin = imin(split * share, tiles), t_end = imin(t_begin + share, tiles);
 
     // query operand: dims 16 f + 8 h .. + 7 (f32: 8 f + 4 h .. + 3) of row i
-    vec_t q[NF];
-    {
+    vec_t q[P::QLDS ? 1 : NF];
+    char* const q_lds = s_buf + P::QAT + (rw * 32 + i) * KSTR + h * 16;
+    if (!P::QLDS || kg == 0) {
         const char* qp = a.q.p + row * a.q.row_bytes + head * a.q.head_bytes;
         // a negative scale is moved into q: the maximum is taken before the scale
         const uint32_t flip = a.sc.negative ? (F32 ? 0x80000000u : 0x80008000u) : 0u;
@@ -217,7 +221,8 @@ __global__ __launch_bounds__(kPreWaves * 64, (PreShape<T, DP, RW>::RESIDENT)) vo
             if (in) w = *reinterpret_cast<const u32x4*>(qp + d * ES);
 #pragma unroll
             for (int e = 0; e < 4; ++e) w[e] ^= flip;
-            q[f] = as_vec<vec_t>(w);
+            if constexpr (P::QLDS) *reinterpret_cast<u32x4*>(q_lds + f * 32) = w;
+            else q[f] = as_vec<vec_t>(w);
         }
     }
     PagedScores sc = a.sc;
@@ -285,17 +290,21 @@ __global__ __launch_bounds__(kPreWaves * 64, (PreShape<T, DP, RW>::RESIDENT)) vo
 #pragma unroll
                 for (int b = 0; b < KB; ++b) s[b] = f32x16{};
 #pragma unroll
-                for (int f = 0; f < NF; ++f)
+                for (int f = 0; f < NF; ++f) {
+                    vec_t qf;
+                    if constexpr (P::QLDS) qf = *reinterpret_cast<const vec_t*>(q_lds + f * 32);
+                    else qf = q[f];
 #pragma unroll
                     for (int b = 0; b < KB; ++b) {
                         const vec_t k = *reinterpret_cast<const vec_t*>(buf + (b * 32 + i) * KSTR + h * 16 + f * 32);
                         if constexpr (F32) {
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) s[b] = mfma_32x32x2(k[e], q[f][e], s[b]);
+                            for (int e = 0; e < 4; ++e) s[b] = mfma_32x32x2(k[e], qf[e], s[b]);
                         } else {
-                            s[b] = mfma_32x32x16(k, q[f], s[b]);
+                            s[b] = mfma_32x32x16(k, qf, s[b]);
                         }
                     }
+                }
                 const bool whole = __all((seen & kAll) == kAll);
                 if constexpr (CAP || BIAS) {
                     const float dist0 = (float)(pos - base - 4 * h);
@@ -380,7 +389,6 @@ __global__ __launch_bounds__(kPreWaves * 64, (PreShape<T, DP, RW>::RESIDENT)) vo
 #pragma unroll
     for (int half = KW / 2; half >= 1; half /= 2) {
         f32x4* at = reinterpret_cast<f32x4*>(s_buf) + (size_t)(kg % half * RW + rw) * (DB * 4 + 1) * 64 + lane;
-        static_assert(KW == 1 || (DB * 4 + 1) * 1024 * (kPreWaves / 2) <= P::LDS, "half the waves' sums fit");
         if (kg >= half && kg < 2 * half) {
 #pragma unroll
             for (int d = 0; d < DB; ++d)
@@ -450,7 +458,6 @@ __global__ __launch_bounds__(kPreWaves * 64, (PreShape<T, DP, RW>::RESIDENT)) vo
     const uint64_t keep = __ballot(live) & ~again;
     // rows through LDS, so that a row leaves in 16-byte pieces side by side (8-byte pieces of
     // 32 rows per store: 6 us for 64 rows of 32 heads instead of 1)
-    static_assert(P::ROWS * (DP * 4 + 16) <= P::LDS, "a workgroup's rows fit its tiles");
     const bool wide = (((uintptr_t)a.out.p | a.out.row_bytes | a.out.head_bytes) & 15) == 0;
     const long long out_at = row * a.out.row_bytes + head * a.out.head_bytes;
     const auto put = [&](auto type) {
@@ -540,7 +547,7 @@ __global__ __launch_bounds__(256) void paged_prefill_join_kernel(PagedAttnArgs a
 
 // A launch of more than the 64 KiB of LDS that a kernel has by default; asked for once per device
 template <auto KERNEL>
-int launch_lds(const PagedAttnArgs& a, dim3 grid, uint32_t lds, hipStream_t st) {
+int launch_lds(const PagedAttnArgs& a, dim3 grid, dim3 block, uint32_t lds, hipStream_t st) {
     static std::atomic<uint64_t> ready{0};
     int dev = 0;
     hipError_t e = hipGetDevice(&dev);
@@ -550,28 +557,32 @@ int launch_lds(const PagedAttnArgs& a, dim3 grid, uint32_t lds, hipStream_t st) 
         if (e == hipSuccess) ready.fetch_or(bit, std::memory_order_relaxed);
     }
     if (e != hipSuccess) return set_error(UOCR_HIP_EHIP, std::string("paged prefill LDS: ") + hipGetErrorString(e));
-    launch_k(KERNEL, grid, dim3(kPreWaves * 64), lds, st, a);
+    launch_k(KERNEL, grid, block, lds, st, a);
     return UOCR_HIP_OK;
 }
 
-template <typename T, int DP, int RW>
-int launch_prefill_rw(const PagedAttnArgs& a, hipStream_t st) {
-    const dim3 grid((unsigned)((long long)a.n_tiles * a.kv_heads * a.n_splits));
-    const uint32_t lds = PreShape<T, DP, RW>::LDS;
+template <typename T, int DP, int RW, int KW>
+int launch_prefill_shape(const PagedAttnArgs& a, hipStream_t st) {
+    typedef PreShape<T, DP, RW, KW> P;
+    const dim3 grid((unsigned)((long long)a.n_tiles * a.kv_heads * a.n_splits)), block(P::WAVES * 64);
     const bool cap = a.sc.cap2 > 0.0f, bias = a.sc.slopes != nullptr;
-    if (cap && bias) return launch_lds<paged_prefill_kernel<T, DP, true, true, RW>>(a, grid, lds, st);
-    if (cap) return launch_lds<paged_prefill_kernel<T, DP, true, false, RW>>(a, grid, lds, st);
-    if (bias) return launch_lds<paged_prefill_kernel<T, DP, false, true, RW>>(a, grid, lds, st);
-    return launch_lds<paged_prefill_kernel<T, DP, false, false, RW>>(a, grid, lds, st);
+    if (cap && bias) return launch_lds<paged_prefill_kernel<T, DP, true, true, RW, KW>>(a, grid, block, P::LDS, st);
+    if (cap) return launch_lds<paged_prefill_kernel<T, DP, true, false, RW, KW>>(a, grid, block, P::LDS, st);
+    if (bias) return launch_lds<paged_prefill_kernel<T, DP, false, true, RW, KW>>(a, grid, block, P::LDS, st);
+    return launch_lds<paged_prefill_kernel<T, DP, false, false, RW, KW>>(a, grid, block, P::LDS, st);
 }
 template <typename T, int DP>
 int launch_prefill_dp(const PagedAttnArgs& a, int rw, hipStream_t st) {
-    if constexpr (DP <= 128) {
-        if constexpr (sizeof(T) == 4)
-            if (rw == 1) return launch_prefill_rw<T, DP, 1>(a, st);
-        if (rw == 2) return launch_prefill_rw<T, DP, 2>(a, st);
+    if constexpr (DP > 128 && sizeof(T) == 2) {
+        return launch_prefill_shape<T, DP, 4, 2>(a, st);
+    } else {
+        if constexpr (DP <= 128) {
+            if constexpr (sizeof(T) == 4)
+                if (rw == 1) return launch_prefill_shape<T, DP, 1, 4>(a, st);
+            if (rw == 2) return launch_prefill_shape<T, DP, 2, 2>(a, st);
+        }
+        return launch_prefill_shape<T, DP, 4, 1>(a, st);
     }
-    return launch_prefill_rw<T, DP, 4>(a, st);
 }
 
 template <typename T>
