@@ -129,14 +129,21 @@ UOCR_HD inline TileWalk tile_walk(const Span& s) {
 // How a decode call is shared out: one workgroup per (sequence, KV head, 16 query heads) where
 // `max_keys` is short or the rows (or the `room` for their keys) too many for the shares' table, else (shares > 0) equal
 // shares of all rows' tiles, one workgroup per share and KV head, and a join.
-// A workgroup of 8 waves takes 8 tiles at a time.
+// A workgroup of 8 waves takes 8 tiles at a time, one of one wave leaves room for seven
+// others: us of 8 / 1 waves: 1128 units of one key 19.3 / 6.1, 640 of up to
+// 120 keys 14.5 / 11.8, 320 of up to 200 12.6 / 16.5.
 struct DecodePlan {
     int blocks;   // of 16 query heads per KV head
+    int unit_waves;
     int shares;   // 0: one workgroup per unit
     unsigned long long records;  // partial results of one (workgroup, first or last sequence, query head) each
 };
 inline DecodePlan paged_decode_plan(long long batch, int heads, int kv_heads, int tile_keys, long long max_keys, long long room) {
-    DecodePlan p{(heads / kv_heads + 15) / 16, 0, 0};
+    DecodePlan p{(heads / kv_heads + 15) / 16, 8, 0, 0};
+    // rounds on the chip (256 workgroups of 8 waves, 2048 of one) times the tiles one after the other, 2 tiles'
+    // time for the beginning and the end
+    const long long units = batch * kv_heads * p.blocks, longest = (max_keys + tile_keys - 1) / tile_keys;
+    if ((units + 2047) / 2048 * (2 + longest) < (units + 255) / 256 * (2 + (longest + 7) / 8)) p.unit_waves = 1;
     if (batch > kPagedShareRows || max_keys <= kPagedUnitTiles * tile_keys) return p;
     const long long kvb = (long long)kv_heads * p.blocks;
     // (a row has two more tiles than its keys fill at most, and the line's length is an int)

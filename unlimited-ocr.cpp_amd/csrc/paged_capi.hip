@@ -113,7 +113,7 @@ int attn_args(const uocr_hip_paged_cache* cache, const uocr_hip_attention_opts* 
     return UOCR_HIP_OK;
 }
 
-// keys that a row may see, as far as the host knows
+// keys that `rows` rows side by side may see, as far as the host knows
 long long most_keys(const PagedAttnArgs& a, int max_kv_len, int rows) {
     long long n = std::min<long long>(a.c.capacity(), INT_MAX);
     if (max_kv_len > 0) n = std::min<long long>(n, max_kv_len);
@@ -172,7 +172,7 @@ int uocr_hip_paged_attention_prefill(const uocr_hip_paged_cache* cache, const uo
     if (!d_q_start) return set_error(UOCR_HIP_EINVAL, "attention: null d_q_start");
     if (opts->window > 0 && !opts->causal) return set_error(UOCR_HIP_EINVAL, "attention: a window needs causal");
     a.q_start = d_q_start;
-    return launch_paged_prefill(a, cache->dtype, most_keys(a, max_kv_len, rows), workspace, workspace_bytes,
+    return launch_paged_prefill(a, cache->dtype, most_keys(a, max_kv_len, std::min(rows, 128 / a.group + 2)), workspace, workspace_bytes,
                                 (hipStream_t)stream);
 }
 

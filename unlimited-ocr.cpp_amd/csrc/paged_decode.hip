@@ -21,9 +21,9 @@
 // have room for it: the result is as exact as with f32 probabilities. A rounding error of 0 makes
 // NaN of an infinite V, so a wave whose sums hold a NaN goes over its keys again without that half.
 //
-// Two ways to share the work, both with workgroups of 8 waves that take a sequence's tiles in turn
+// Two ways to share the work, with workgroups of 8 waves that take a sequence's tiles in turn
 // and are combined in LDS:
-//   * short caches: a workgroup per (sequence, KV head);
+//   * short caches: a workgroup per (sequence, KV head), of one wave where there are many;
 //   * else all sequences' tiles are one line, cut into equal shares whatever the
 //     lengths: a workgroup per (share, KV head), its KV heads' neighbours beside it (their rows are
 //     side by side in memory). Of a sequence that several shares cut, each leaves its sums (at most
@@ -344,10 +344,9 @@ __device__ __forceinline__ f32x4 combine(const DecodeLds<UW>& s, const float* o,
     return r;
 }
 
-// One (sequence, KV head, 16 query heads) per workgroup
-template <typename T, int DP, bool CAP, bool BIAS>
-__global__ __launch_bounds__(kDecWaves<DP> * 64) void paged_decode_unit_kernel(PagedAttnArgs a) {
-    constexpr int UW = kDecWaves<DP>;
+// One (sequence, KV head, 16 query heads) per workgroup of UW waves
+template <typename T, int DP, bool CAP, bool BIAS, int UW>
+__global__ __launch_bounds__(UW * 64) void paged_decode_unit_kernel(PagedAttnArgs a) {
     typedef DecodeWave<T, DP, CAP, BIAS> W;
     __shared__ DecodeLds<UW> s_w;
     extern __shared__ __attribute__((aligned(16))) float s_o[];
@@ -664,6 +663,17 @@ __global__ __launch_bounds__(kJoinThreads) void paged_decode_join_kernel(PagedAt
     }
 }
 
+template <typename T, int DP, int UW>
+void launch_unit(const PagedAttnArgs& a, hipStream_t st) {
+    const bool cap = a.sc.cap2 > 0.0f, bias = a.sc.slopes != nullptr;
+    const dim3 grid((unsigned)a.batch * a.kv_heads * ((a.group + kDecCols - 1) / kDecCols)), block(UW * 64);
+    const uint32_t lds = UW * std::min(a.group, kDecCols) * (DP + 4) * sizeof(float);
+    if (cap && bias) launch_k(paged_decode_unit_kernel<T, DP, true, true, UW>, grid, block, lds, st, a);
+    else if (cap) launch_k(paged_decode_unit_kernel<T, DP, true, false, UW>, grid, block, lds, st, a);
+    else if (bias) launch_k(paged_decode_unit_kernel<T, DP, false, true, UW>, grid, block, lds, st, a);
+    else launch_k(paged_decode_unit_kernel<T, DP, false, false, UW>, grid, block, lds, st, a);
+}
+
 template <typename T, int DP>
 void launch_dp(const PagedAttnArgs& a, hipStream_t st) {
     const int kvb = a.kv_heads * ((a.group + kDecCols - 1) / kDecCols);
@@ -672,11 +682,8 @@ void launch_dp(const PagedAttnArgs& a, hipStream_t st) {
     // (the join takes 16 bytes per thread)
     const uint32_t lds = std::max<uint32_t>(kDecWaves<DP> * std::min(a.group, kDecCols) * (DP + 4) * sizeof(float), block.x * 16);
     if (!a.n_splits) {
-        const dim3 grid((unsigned)a.batch * kvb);
-        if (cap && bias) launch_k(paged_decode_unit_kernel<T, DP, true, true>, grid, block, lds, st, a);
-        else if (cap) launch_k(paged_decode_unit_kernel<T, DP, true, false>, grid, block, lds, st, a);
-        else if (bias) launch_k(paged_decode_unit_kernel<T, DP, false, true>, grid, block, lds, st, a);
-        else launch_k(paged_decode_unit_kernel<T, DP, false, false>, grid, block, lds, st, a);
+        if (a.unit_waves == 1) launch_unit<T, DP, 1>(a, st);
+        else launch_unit<T, DP, kDecWaves<DP>>(a, st);
         return;
     }
     const dim3 grid((unsigned)a.n_splits * kvb);
@@ -700,6 +707,7 @@ int launch_paged_decode(PagedAttnArgs a, int dtype, long long max_keys, void* ws
     const DecodePlan p = paged_decode_plan(a.batch, a.heads, a.kv_heads, dtype == UOCR_HIP_DTYPE_F32 ? 16 : 32, max_keys,
                                            std::min<long long>(a.c.capacity(), INT_MAX));
     a.n_splits = p.shares;
+    a.unit_waves = p.unit_waves;
     if ((long long)a.batch * a.kv_heads * p.blocks >= 1 << 23)  // (a launch has fewer than 2^32 threads)
         return set_error(UOCR_HIP_EUNSUPPORTED, "attention: batch too large");
     if (p.shares)

@@ -44,6 +44,7 @@ struct PagedAttnArgs {
     int* counters;   // (decode) [batch][KV heads x blocks of 16 heads]: sums that are there (0 between calls);
                      // the workspace's first word before them. Null: joined by a kernel of its own
     int* part_rows;  // (decode) [batch][2]: first and last share with tiles of a row
+    int unit_waves;  // (decode) waves of such a workgroup: 1, or as many as there are
     int n_tiles;   // (prefill) query tiles that the grid has room for
 };
 
