@@ -248,15 +248,17 @@ __global__ __launch_bounds__(RW * KW * 64, (PreShape<T, DP, RW, KW>::PER_SIMD)) 
 #pragma unroll
         for (int e = 0; e < NL; ++e) {
             const int u = e * GT + gtid, r = u / CH, c = u % CH;
-            const long long at = shfl64(off, r) + c * 16;
-            kw[e] = vw[e] = u32x4{0, 0, 0, 0};
-            if (c * (16 / ES) < a.head_dim) {
-                kw[e] = *reinterpret_cast<const u32x4*>(kbase + at);
-                vw[e] = *reinterpret_cast<const u32x4*>(vbase + at);
-            }
+            const long long at = shfl64(off, r) + imin(c, a.head_dim * ES / 16 - 1) * 16;
+            kw[e] = *reinterpret_cast<const u32x4*>(kbase + at);
+            vw[e] = *reinterpret_cast<const u32x4*>(vbase + at);
         }
     };
     auto store = [&](char* buf) {
+        if (a.head_dim < DP) {  // 0 past the head
+#pragma unroll
+            for (int e = 0; e < NL; ++e)
+                if ((e * GT + gtid) % CH * (16 / ES) >= a.head_dim) kw[e] = vw[e] = u32x4{0, 0, 0, 0};
+        }
 #pragma unroll
         for (int e = 0; e < NL; ++e) {
             const int u = e * GT + gtid, r = u / CH, c = u % CH;
@@ -316,7 +318,9 @@ __global__ __launch_bounds__(RW * KW * 64, (PreShape<T, DP, RW, KW>::PER_SIMD)) 
                 }
                 constexpr bool kScaled = CAP || BIAS;
                 if (!whole) {
-                    const uint64_t mine = seen >> (4 * h);
+                    uint64_t mine = seen >> (4 * h);
+                    // (a branch: as selects it would be a third of the loop's vector instructions)
+                    asm volatile("" : "+v"(mine));
 #pragma unroll
                     for (int b = 0; b < KB; ++b)
 #pragma unroll
