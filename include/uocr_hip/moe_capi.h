@@ -584,7 +584,8 @@ typedef struct {
  * with heads of 256. A workspace is set up once, by _workspace_init, before its first call, and again if a call
  * on it was cut short; calls leave it ready for the next, of any shape that it is large enough for. Calls that
  * overlap in time need a workspace each, two captured graphs that may run at the same time too. A decode
- * call on one that was not set up gives NaN. */
+ * call on one that was not set up gives NaN. Calls whose keys are not split do without one (NULL); which are
+ * depends on sizes and options, and the others refuse (UOCR_HIP_EWORKSPACE). */
 size_t uocr_hip_paged_attention_workspace_size(const uocr_hip_paged_cache* cache, int heads, int rows);
 int uocr_hip_paged_attention_workspace_init(void* workspace, size_t workspace_bytes, void* stream);
 
@@ -608,7 +609,8 @@ int uocr_hip_paged_attention_decode(const uocr_hip_paged_cache* cache, const uoc
  * in the cache already: row i of n is position kv_len[s] - n + i. d_q_start has batch + 1 entries, not
  * falling; rows outside all of them, and rows of an s not in [0, n_seqs), are left as they were. Rows before position 0 (more
  * rows than kv_len) give zeros. The rest as for the decode call, except that for bf16 and f16 the
- * probabilities are rounded to that type (relative 2^-9, 2^-12) before they meet V. */
+ * probabilities are rounded to that type before they meet V (relative 2^-8, 2^-11; f16's below 2^-14 by at most
+ * 2^-25 of the row's largest). */
 int uocr_hip_paged_attention_prefill(const uocr_hip_paged_cache* cache, const uocr_hip_attention_opts* opts,
                                      const uocr_hip_rows* q, int rows, int batch, const int* d_q_start,
                                      const int* d_seqs, const int* d_kv_len, int max_kv_len, const uocr_hip_rows* out,

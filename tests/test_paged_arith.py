@@ -131,6 +131,13 @@ static int splits() {
                             CHECK(p.row_waves == 4 || p.row_waves == 2 || p.row_waves == 1);
                             CHECK(p.tiles * p.row_waves * 32 >= r * g && p.splits >= 1 && p.splits <= kPagedMaxSplits);
                             if (p.splits > 1) CHECK((unsigned long long)r * kv * g * p.splits <= most);
+                            // several entries, whose rows all see some of the keys
+                            for (long long batch : {2ll, 7ll, r}) for (long long least : {0ll, keys / 2, keys}) {
+                                const PrefillPlan b = paged_prefill_plan(r, batch, kv * g, kv, d, f32, keys, least);
+                                CHECK(b.row_waves == 4 || b.row_waves == 2 || b.row_waves == 1);
+                                CHECK(b.tiles >= r * g / (b.row_waves * 32) + batch && b.splits >= 1 && b.splits <= kPagedMaxSplits);
+                                if (b.splits > 1) CHECK((unsigned long long)r * kv * g * b.splits <= most);
+                            }
                         }
                     }
     return 0;

@@ -19,7 +19,7 @@ constexpr int kPagedCounters = 16384;   // (sequence, KV head, 16 query heads) o
 constexpr int kPagedMagic = 0x70616765; // first word of a workspace that was set up
 constexpr int kPagedHead = 64 + kPagedCounters * 4;  // bytes before a workspace's partial results
 constexpr int kPagedUnitTiles = 8;     // tiles of keys that one workgroup takes alone
-constexpr int kPagedPrefillTarget = 1024;  // workgroups of a split prefill call at most
+constexpr int kPagedPrefillTarget = 1024;  // workgroups of 128 pairs of a split prefill call at most
 constexpr int kPagedMaxSplits = 128;
 
 // n / d for 0 <= n < 2^31 by a multiplication: with s = ceil(log2 d) and
@@ -157,55 +157,70 @@ inline DecodePlan paged_decode_plan(long long batch, int heads, int kv_heads, in
     return p;
 }
 
-// How a prefill call is shared out: workgroups of 4 waves, `row_waves` of them along the (row, head)
-// pairs of a KV head (32 each), the others on other tiles of keys; `tiles` of pairs per KV head at
-// most (each entry rounds up by less than one); the keys split over `splits` workgroups where
-// those leave some of the chip idle, 256 keys in each at least (64 rows of 32 heads on 16000 keys: 1 split 351 us,
-// 3 129, 12 61; 1024 rows of 16 heads of 256: 1 69, 2 56, 3 65).
+// How a prefill call is shared out: workgroups of 4 waves (16-bit heads above 128: 8), `row_waves` of them along the
+// (row, head) pairs of a KV head (32 each), the others on other tiles of keys; `tiles` of pairs per KV head at
+// most (each entry rounds up by less than one), each of which sees min_keys to max_keys keys; the keys split over
+// `splits` workgroups, 256 keys in each at least. Taken is what costs the least by this model, in quarters of the
+// time that a tile of keys (64; f32: 32) takes a workgroup of 128 pairs on a full chip:
+//   * a tile of keys, and a workgroup's beginning and end, by shape, below;
+//   * rounds of `slots` workgroups; where they fill the chip the longest go first, and what the last round
+//     leaves idle is as long as the shortest;
+//   * splits: their sums' way through memory, a join with its launch.
 // 128 pairs per workgroup share K and V best, 64 or 32 leave fewer rounds one after the other and more
-// workgroups: they are for calls that do not fill the chip, and need keys for every wave. us with 4 / 2 / 1 row
-// waves, head_dim 128 (workgroups of 128 pairs):
-//   bf16  10 heads, 64 rows (10) 8.2 / 9.9 / 12.1, 256 (30) 14.2 / 12.8 / 12.7, 1024 (90) 36 / 31 / 29,
-//         4096 (330) 133 / 102 / 198; 32 heads over 8, 1024 rows (264) 39 / 32 / 70, 4096 (1032) 191 / 239 / 583
-//   f32   10 heads, 64 rows 17.0 / 14.7 / 16.3, 256 47 / 34 / 24, 1024 93 / 77 / 65, 4096 718 / 594 / 589;
-//         32 heads over 8, 1024 rows 166 / 135 / 153, 4096 1238 / 1322 / 1770
-// Heads above 128 have no room for it (registers, LDS).
+// workgroups. us with 4 / 2 / 1 row waves, head_dim 128 (workgroups of 128 pairs):
+//   bf16  10 heads, 64 rows (10) 7.5 / 9.0, 256 (30) 13.2 / 11.6, 1024 (90) 35 / 30, 4096 (330) 126 / 97;
+//         32 heads over 8, 1024 rows (264) 51 / 30, 4096 (1032) 188 / 227, 1100 on 16000 keys (280) 456 / 711
+//   f32   10 heads, 64 rows 16.4 / 13.9 / 15.5, 256 46 / 30 / 23, 1024 91 / 65 / 64, 4096 481 / 470 / 565;
+//         32 heads over 8, 1024 rows 169 / 121 / 147, 4096 1230 / 1201 / 1720
+// Heads above 128 have no room for it (registers, LDS) and keep 4. Splits, bf16: 64 rows of 32 heads on 16000 keys
+// 1 split 351 us, 3 129, 12 61; 2100 rows of 16 heads of 256 (264 workgroups) on 20000 keys 1 1785, 2 1345, 3 1211.
 struct PrefillPlan {
     int row_waves, splits;
     long long tiles;
 };
 inline PrefillPlan paged_prefill_plan(long long rows, long long batch, int heads, int kv_heads, int head_dim, bool f32,
-                                      long long max_keys) {
+                                      long long max_keys, long long min_keys = 0) {
+    struct Shape {
+        int row_waves, slots;
+        double tile, ends, way;
+    };
+    constexpr Shape kShapes[] = {{4, 512, 4.0, 16.0, 12.0}, {2, 512, 2.4, 18.0, 6.0},   // 16 bits, heads up to 128
+                                 {4, 256, 4.0, 16.0, 12.0},                             // above
+                                 {2, 256, 2.0, 7.0, 3.5},   {1, 256, 1.2, 11.0, 1.7},   // f32
+                                 {4, 256, 4.0, 6.0, 7.0}};
+    const int first = (f32 ? 3 : 0) + (head_dim > 128 ? 2 : 0), last = head_dim > 128 ? first : first + 1;
     const long long pairs = rows * (heads / kv_heads);
-    const auto tiles = [&](int rw) { return pairs / (32 * rw) + batch; };
-    const auto groups = [&](int rw) { return tiles(rw) * kv_heads; };
+    const double longest = (double)max_keys / (f32 ? 32 : 64), shortest = (double)min_keys / (f32 ? 32 : 64);
     PrefillPlan p{4, 1, 0};
-    if (head_dim <= 128) {
-        if (f32 && groups(1) < 512 && max_keys > 96) p.row_waves = 1;
-        else if (groups(4) < (f32 ? 1024 : 512) && max_keys > (f32 ? 32 : 64)) p.row_waves = 2;
-    }
-    p.tiles = tiles(p.row_waves);
-    // Splits: the fewest rounds of tiles one after the other, with 4 tiles' time for a workgroup's
-    // beginning and end and for the join. `units`: the workgroups there are likely to be.
-    const long long slots = head_dim > 128 || p.row_waves == 1 ? 256 : 512;
-    long long per_kv = batch == 1 ? (pairs + 32 * p.row_waves - 1) / (32 * p.row_waves) : pairs / (32 * p.row_waves) + (batch + 1) / 2;
-    if (per_kv < batch) per_kv = batch;
-    const long long units = per_kv * kv_heads, keys = f32 ? 32 : 64, most = max_keys / 256;
-    if (units >= slots) return p;
-    long long best = 1ll << 62;
-    for (long long n = 1; n <= kPagedMaxSplits && (n == 1 || (n <= most && units * n <= kPagedPrefillTarget)); ++n) {
-        const long long rounds = (units * n + slots - 1) / slots, cost = rounds * (4 * max_keys / (keys * n) + 16) + (n > 1 ? 16 + n : 0);
-        if (cost < best) {
-            best = cost;
-            p.splits = (int)n;
+    double best = 1e300;
+    for (int k = first; k <= last; ++k) {
+        const Shape& s = kShapes[k];
+        const long long across = 32 * s.row_waves;
+        // the workgroups that there are likely to be
+        long long units = batch == 1 ? (pairs + across - 1) / across : pairs / across + (batch + 1) / 2;
+        units = (units < batch ? batch : units) * kv_heads;
+        const bool full = units >= s.slots;
+        const double mean = full ? (longest + shortest) / 2 : longest, least = full ? shortest : longest;
+        for (long long n = 1; n <= kPagedMaxSplits; ++n) {
+            if (n > 1 && (n > max_keys / 256 || units * n * s.row_waves > 4 * kPagedPrefillTarget)) break;
+            const double turns = (double)(units * n) / s.slots;
+            const long long whole = (units * n + s.slots - 1) / s.slots;
+            double cost = turns * (s.tile * mean / n + s.ends) + (whole - turns) * (s.tile * least / n + s.ends);
+            if (n > 1) cost += (f32 ? 6.0 + 0.3 * n : 16.0 + 0.5 * n) + whole * s.way * (full ? 2 : 1);
+            if (cost < best) {
+                best = cost;
+                p.row_waves = s.row_waves;
+                p.splits = (int)n;
+            }
         }
     }
+    p.tiles = pairs / (32 * p.row_waves) + batch;
     return p;
 }
 
 // Partial results that calls of up to `rows` rows may hold. Decode: 2 per workgroup and query head;
-// prefill: a unit is 128 (row, head) pairs of a KV head at most, and units * splits stays below
-// kPagedPrefillTarget.
+// prefill: a unit is 32 (row, head) pairs of a KV head per row wave at most, and units * splits * row waves
+// stays within 4 kPagedPrefillTarget.
 inline unsigned long long paged_workspace_records(long long rows, int heads, int kv_heads) {
     const long long group = heads / kv_heads, kvb = kv_heads * ((group + 15) / 16), cols = group < 16 ? group : 16;
     const long long decode = (kPagedShareGroups + kvb) * 2 * cols;

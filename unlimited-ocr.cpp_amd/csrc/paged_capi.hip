@@ -172,8 +172,11 @@ int uocr_hip_paged_attention_prefill(const uocr_hip_paged_cache* cache, const uo
     if (!d_q_start) return set_error(UOCR_HIP_EINVAL, "attention: null d_q_start");
     if (opts->window > 0 && !opts->causal) return set_error(UOCR_HIP_EINVAL, "attention: a window needs causal");
     a.q_start = d_q_start;
-    return launch_paged_prefill(a, cache->dtype, most_keys(a, max_kv_len, std::min(rows, 128 / a.group + 2)), workspace, workspace_bytes,
-                                (hipStream_t)stream);
+    const long long most = most_keys(a, max_kv_len, std::min(rows, 128 / a.group + 2));
+    // the first of an entry's rows, of entries of equal length
+    long long least = most_keys(a, max_kv_len, INT_MAX) - (opts->causal ? rows / batch : 0);
+    least = std::max(std::min(least, most), 0ll);
+    return launch_paged_prefill(a, cache->dtype, most, least, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -20,9 +20,9 @@ int paged_cache(const uocr_hip_paged_cache* c, PagedCache* out);  // paged_capi.
 // Rows of `heads` heads, checked; `vec`: 16-byte alignment needed
 int paged_rows(const char* what, const uocr_hip_rows* r, bool vec, PagedRows* out);
 
-// max_keys: what a row may see, as far as the host knows. UOCR_HIP_OK or a code with its message.
+// max_keys: what a row may see, min_keys: what the rows of an entry that fills many tiles all see, as far as the host knows. UOCR_HIP_OK or a code with its message.
 int launch_paged_decode(PagedAttnArgs a, int dtype, long long max_keys, void* ws, size_t ws_bytes, hipStream_t st);
-int launch_paged_prefill(PagedAttnArgs a, int dtype, long long max_keys, void* ws, size_t ws_bytes, hipStream_t st);
+int launch_paged_prefill(PagedAttnArgs a, int dtype, long long max_keys, long long min_keys, void* ws, size_t ws_bytes, hipStream_t st);
 
 // Gives a call its place for `records` partial results and (decode) `rows` entries about rows
 int paged_take_workspace(PagedAttnArgs& a, size_t records, int rows, void* ws, size_t ws_bytes);

@@ -3,8 +3,10 @@
 
 namespace uocr_hip {
 
-int launch_paged_prefill(PagedAttnArgs a, int dtype, long long max_keys, void* ws, size_t ws_bytes, hipStream_t st) {
-    const PrefillPlan p = paged_prefill_plan(a.rows, a.batch, a.heads, a.kv_heads, a.head_dim, dtype == UOCR_HIP_DTYPE_F32, max_keys);
+int launch_paged_prefill(PagedAttnArgs a, int dtype, long long max_keys, long long min_keys, void* ws, size_t ws_bytes,
+                         hipStream_t st) {
+    const PrefillPlan p = paged_prefill_plan(a.rows, a.batch, a.heads, a.kv_heads, a.head_dim, dtype == UOCR_HIP_DTYPE_F32,
+                                             max_keys, min_keys);
     if (p.tiles * a.kv_heads * p.splits >= 1 << 23)  // (a launch has fewer than 2^32 threads)
         return set_error(UOCR_HIP_EUNSUPPORTED, "attention: too many rows or entries");
     a.n_tiles = (int)p.tiles;

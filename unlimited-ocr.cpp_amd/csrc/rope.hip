@@ -5,7 +5,8 @@
 // 0.03 rad at position 10^6), sine and cosine of that are f32. Bound by the bytes: each
 // element is read and written once; the sines of a row are computed once in LDS for all
 // heads. One workgroup per row: 8 elements (16-byte accesses for 16-bit types) per thread and
-// step, the rotated half and its partner in one thread, so q_out may be q.
+// step, the rotated half and its partner in one thread, so q_out may be q. 8192 rows of 48 heads of
+// 128: bf16 32 us, 6.2 TB/s read and written; f32 79 us, 5.1.
 #include <hip/hip_runtime.h>
 
 #include <initializer_list>
@@ -153,7 +154,7 @@ bool aligned16(const PagedRows& r) { return !((uintptr_t)r.p % 16 || r.row_bytes
 
 int launch_rope(const RopeArgs& a, int from, int to, bool vec, hipStream_t st) {
     // 8 elements at a time where the pairs divide and every place is 16-byte aligned
-    // (8192 rows of 48 heads of 128 in bf16, one element at a time: see below)
+    // (8192 rows of 48 heads of 128: bf16 32 us, 61 one at a time; f32 79 and 94)
     const int half = a.rotary / 2;
     vec = vec && a.head_dim % 8 == 0 && half % 8 == 0;
     if (from == UOCR_HIP_DTYPE_F32) launch_to<float>(a, to, vec, st);

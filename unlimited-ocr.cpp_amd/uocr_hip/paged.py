@@ -125,7 +125,8 @@ def attention_decode(q, cache, kv_len, out, seqs=None, scale=None, softcap=0.0, 
     """Attention of one new token per sequence: row b of q and out [batch, heads, head_dim] is the
     last position of sequence seqs[b] (b if None), its K and V in the cache already. kv_len and
     prefix_len [n_seqs] int32; see uocr_hip_attention_opts for the scores and masks.
-    max_kv_len (0: the table's room) only chooses the split."""
+    max_kv_len (0: the table's room) only chooses the split. workspace: from attention_workspace, for as
+    many rows; without one, calls that are split are refused."""
     _call(_n.attention, cache.index, stream,
           (q, cache.address, cache.index, None, kv_len, out, seqs, True, scale, softcap, slopes, window, prefix_len, False,
            key_begin, key_end, max_kv_len, workspace))
