@@ -5,8 +5,7 @@
 // keys with a running maximum and sum per row. 4 head_dim operations per visible pair and head
 // on the matrix cores, beside which a score costs some 4 vector instructions (scale, exponential,
 // sum, rounding). 8192 rows of 32 heads of 128 over 8, causal, bf16: 655 us, 839 TFLOP/s; the matrix cores
-// are busy for 39% of the cycles, the vector units for 60, LDS for 35, bank conflicts below 1, 76 MB from
-// memory. f32, 4096 rows of 10 heads: 470 us, 91 TFLOP/s.
+// are busy for 39% of the cycles, the vector units for 47, LDS for 35, bank conflicts below 1. f32, 4096 rows of 10 heads: 470 us, 91 TFLOP/s.
 //
 // A workgroup of 4 waves takes 128 query rows of one KV head (64 or 32 in small calls, the waves
 // then also taking turns at the tiles of keys): the `group` query heads that
