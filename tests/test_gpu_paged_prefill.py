@@ -228,3 +228,71 @@ def test_prefill_captured_and_on_another_stream(dev):
     assert torch.equal(out, eager)
     paged().attention_prefill(q, cache, starts, kv, q, workspace=ws)  # out may be q
     assert torch.equal(q, eager)
+
+
+@pytest.mark.parametrize("dtype,rows,heads,d", [("bf16", 1, 1, 64), ("f32", 3, 2, 40), ("bf16", 2, 2, 256)])
+def test_prefill_many_splits(dev, dtype, rows, heads, d):
+    """Few rows over tens of thousands of keys: more splits than a wave has lanes, some of them without a key
+    that the row sees; values that are not finite in hidden places, and an infinite one that all see."""
+    print(f"[prefill splits] {dtype} {rows}x{heads}x{d}", flush=True)
+    n, rng = 120001 if d <= 64 else 33001, np.random.default_rng(d)
+    pool = R.Pool(rng, [n, 20], 1, d, 64, dtype, dev)
+    q = [rows, rows]
+    run_prefill(dev, rng, pool, q, heads)
+    run_prefill(dev, rng, pool, q, heads, window=700, prefix_len=[130, 4])
+    run_prefill(dev, rng, pool, q, heads, key_begin=[20000] * rows + [30] * rows, softcap=20.0)  # (the second sees nothing)
+    pool.poison(0, 19999)
+    pool.table[0, 3] = -1
+    run_prefill(dev, rng, pool, q, heads, key_begin=[20000] * rows + [5] * rows)
+    pool.v_pages[int(pool.table[0, 400]), 0, 0, 1] = float("inf")
+    cache = pool.cache()
+    qd = rand(rng, 2 * rows, heads, d).to(R.DT[dtype]).to(dev)
+    out = torch.zeros_like(qd)
+    paged().attention_prefill(qd, cache, i32([0, rows, 2 * rows], dev), pool.kv_len, out, key_begin=i32([20000] * 2 * rows, dev),
+                              workspace=paged().attention_workspace(cache, heads, 2 * rows))
+    assert (out[:rows, :, 1].float() == float("inf")).all() and (out[rows:] == 0).all()
+    out[:rows, :, 1] = 0
+    assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,d", [("bf16", 2, 1, 256), ("f32", 1, 1, 136), ("bf16", 6, 3, 64)])
+def test_prefill_splits_of_a_full_chip(dev, dtype, heads, kv_heads, d):
+    """More entries than the chip takes at once, three of them long: split in rounds, most splits empty."""
+    print(f"[prefill full] {dtype} {heads}/{kv_heads}x{d}", flush=True)
+    rng = np.random.default_rng(heads + d)
+    lens = [int(x) for x in rng.integers(0, 40, 270)]
+    for b, n in ((0, 6000), (130, 5003), (269, 6000)):
+        lens[b] = n
+    q = [1 + b % 3 for b in range(270)]
+    at = np.concatenate([[0], np.cumsum(q)])
+    pool = R.Pool(rng, lens, kv_heads, d, 16, dtype, dev)
+    check = {int(at[b]) + i for b in (0, 1, 2, 64, 129, 130, 131, 200, 268, 269) for i in range(q[b])}
+    for kw in (dict(), dict(window=3000), dict(causal=False)):
+        run_prefill(dev, rng, pool, q, heads, check=check, max_kv_len=6000, **kw)
+
+
+def test_prefill_split_captured(dev):
+    """A captured call that splits its keys, replayed between others on the same workspace and with other lengths."""
+    rng = np.random.default_rng(3)
+    pool = R.Pool(rng, [5000, 4000], 2, 64, 16, "bf16", dev)
+    cache = pool.cache()
+    q = rand(rng, 12, 4, 64, std=1.5).to(torch.bfloat16).to(dev)
+    start, out, ws = i32([0, 5, 12], dev), torch.zeros_like(q), paged().attention_workspace(cache, 4, 12)
+
+    def call(o):
+        paged().attention_prefill(q, cache, start, pool.kv_len, o, max_kv_len=5000, workspace=ws)
+
+    call(out)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call(out)
+    for lens in ([5000, 4000], [9, 3999], [5, 7], [4999, 0], [5000, 4000]):
+        pool.kv_len.copy_(i32(lens, dev))
+        want = torch.zeros_like(q)
+        call(want)
+        paged().attention_decode(q[:2], cache, pool.kv_len, torch.zeros_like(q[:2]), max_kv_len=5000, workspace=ws)
+        out.fill_(3.0)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
