@@ -172,8 +172,11 @@ inline DecodePlan paged_decode_plan(long long batch, int heads, int kv_heads, in
 //         32 heads over 8, 1024 rows (264) 51 / 30, 4096 (1032) 188 / 227, 1100 on 16000 keys (280) 456 / 711
 //   f32   10 heads, 64 rows 16.4 / 13.9 / 15.5, 256 46 / 30 / 23, 1024 91 / 65 / 64, 4096 481 / 470 / 565;
 //         32 heads over 8, 1024 rows 169 / 121 / 147, 4096 1230 / 1201 / 1720
-// Heads above 128 have no room for it (registers, LDS) and keep 4. Splits, bf16: 64 rows of 32 heads on 16000 keys
-// 1 split 351 us, 3 129, 12 61; 2100 rows of 16 heads of 256 (264 workgroups) on 20000 keys 1 1785, 2 1345, 3 1211.
+// Heads above 128 keep 4 where they fill the chip (64 pairs: one wave per SIMD, bf16 376 us instead of 216 for 4096
+// rows of 16 heads of 256 over 4); smaller calls of those heads: 64 rows bf16 16.9 / 13.2, f32 32 / 31, 256 rows 24 / 21
+// and 91 / 77, heads of 192 in f32 26 / 22 and 70 / 47 (in 16 bits 64 pairs gain nothing there: 11.3 / 11.9).
+// Splits, bf16: 64 rows of 32 heads on 16000 keys 1 split 351 us, 3 129, 12 61; 2100 rows of 16 heads of 256 (264
+// workgroups) on 20000 keys 1 1785, 2 1345, 3 1211.
 struct PrefillPlan {
     int row_waves, splits;
     long long tiles;
@@ -185,10 +188,11 @@ inline PrefillPlan paged_prefill_plan(long long rows, long long batch, int heads
         double tile, ends, way;
     };
     constexpr Shape kShapes[] = {{4, 512, 4.0, 16.0, 12.0}, {2, 512, 2.4, 18.0, 6.0},   // 16 bits, heads up to 128
-                                 {4, 256, 4.0, 16.0, 12.0},                             // above
+                                 {4, 256, 4.0, 16.0, 12.0}, {2, 256, 4.2, 12.0, 6.0},   // above
                                  {2, 256, 2.0, 7.0, 3.5},   {1, 256, 1.2, 11.0, 1.7},   // f32
-                                 {4, 256, 4.0, 6.0, 7.0}};
-    const int first = (f32 ? 3 : 0) + (head_dim > 128 ? 2 : 0), last = head_dim > 128 ? first : first + 1;
+                                 {4, 256, 4.0, 6.0, 7.0},   {2, 256, 3.0, 5.0, 3.5}};
+    const int first = (f32 ? 4 : 0) + (head_dim > 128 ? 2 : 0);
+    const int last = !f32 && head_dim > 128 && head_dim <= 192 ? first : first + 1;
     const long long pairs = rows * (heads / kv_heads);
     const double longest = (double)max_keys / (f32 ? 32 : 64), shortest = (double)min_keys / (f32 ? 32 : 64);
     PrefillPlan p{4, 1, 0};
@@ -200,6 +204,7 @@ inline PrefillPlan paged_prefill_plan(long long rows, long long batch, int heads
         long long units = batch == 1 ? (pairs + across - 1) / across : pairs / across + (batch + 1) / 2;
         units = (units < batch ? batch : units) * kv_heads;
         const bool full = units >= s.slots;
+        if (full && k > first && head_dim > 128) continue;
         const double mean = full ? (longest + shortest) / 2 : longest, least = full ? shortest : longest;
         for (long long n = 1; n <= kPagedMaxSplits; ++n) {
             if (n > 1 && (n > max_keys / 256 || units * n * s.row_waves > 4 * kPagedPrefillTarget)) break;

@@ -10,7 +10,7 @@
 // A workgroup of 4 waves takes 128 query rows of one KV head (64 or 32 in small calls, the waves
 // then also taking turns at the tiles of keys): the `group` query heads that
 // share it side by side for each token, so that K and V tiles serve all of them. 16-bit heads above 128
-// take 8 waves, two per SIMD, in two turns at the keys. Tiles of 64 keys (32 for f32 and for 8 waves) go
+// take 8 waves, two per SIMD, in two turns at the keys, where they fill the chip. Tiles of 64 keys (32 for f32 and for heads above 128) go
 // through registers into LDS, the next one in flight during the current one's products; registers (and not a
 // direct load) because pages may start anywhere and rows are padded. Each wave has 32 rows:
 //   * S^T = K Q^T on v_mfma_f32_32x32x16: lane (i, h) = (lane % 32, lane / 32) holds row i's
@@ -41,7 +41,7 @@ template <typename T, int DP, int RW, int KW>
 struct PreShape {
     static constexpr int ES = sizeof(T), WAVES = RW * KW;
     static constexpr int ROWS = RW * 32;  // packed query rows per workgroup
-    static constexpr int KEYS = ES == 4 || WAVES == 8 ? 32 : 64;  // per tile
+    static constexpr int KEYS = ES == 4 || DP > 128 ? 32 : 64;  // per tile
     static constexpr int KSTR = DP * ES + 16;
     static constexpr int VPAD = ES == 4 ? 32 : (DP * 2 % 256 == 64 || DP * 2 % 256 == 192) ? 0 : 64;
     static constexpr int VSTR = DP * ES + VPAD;
@@ -614,16 +614,14 @@ int launch_prefill_shape(const PagedAttnArgs& a, hipStream_t st) {
 }
 template <typename T, int DP>
 int launch_prefill_dp(const PagedAttnArgs& a, int rw, hipStream_t st) {
-    if constexpr (DP > 128 && sizeof(T) == 2) {
-        return launch_prefill_shape<T, DP, 4, 2>(a, st);
-    } else {
-        if constexpr (DP <= 128) {
-            if constexpr (sizeof(T) == 4)
-                return rw == 1 ? launch_prefill_shape<T, DP, 1, 4>(a, st) : launch_prefill_shape<T, DP, 2, 2>(a, st);
-            else if (rw == 2) return launch_prefill_shape<T, DP, 2, 2>(a, st);
-        }
-        if constexpr (DP > 128 || sizeof(T) == 2) return launch_prefill_shape<T, DP, 4, 1>(a, st);
-    }
+    constexpr bool F32 = sizeof(T) == 4;
+    if constexpr (F32 && DP <= 128)
+        if (rw == 1) return launch_prefill_shape<T, DP, 1, 4>(a, st);
+    if constexpr (F32 || DP <= 128 || DP > 192)
+        if (rw == 2) return launch_prefill_shape<T, DP, 2, 2>(a, st);
+    if constexpr (!F32 && DP > 128) return launch_prefill_shape<T, DP, 4, 2>(a, st);
+    else if constexpr (!F32 || DP > 128) return launch_prefill_shape<T, DP, 4, 1>(a, st);
+    else return set_error(UOCR_HIP_EINVAL, "attention: no such shape");  // (f32 up to 128 plans 1 or 2)
 }
 
 template <typename T>
